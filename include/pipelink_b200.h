@@ -539,6 +539,59 @@ int plb_tp_gemm_bf16(const void* a_bf16, const void* b_bf16, const int32_t* bloc
                      const uint32_t* ready, uint32_t ready_target, void* out_bf16, void* const* out_peers,
                      plb_status* status, void* stream);
 
+/* ------------------------------------------------------------------ prefill attention, backward
+ * Gradients of plb_attention_fwd's causal attention (same scale, window and softcap arguments): q, out, d_out, dq
+ * bf16 [batch, seq, q_heads, 128]; k, v, dk, dv bf16 [batch, seq, kv_heads, 128]; lse f32 [batch * q_heads, seq] as
+ * the forward call wrote it. All contiguous and 16-byte aligned; any seq >= 1 (rows past a sequence's end are
+ * neither read as keys nor written). The probabilities are recomputed from lse; dk and dv are summed over the
+ * query heads of their group in fp32 and rounded once, with no atomics: the same inputs give the same bits.
+ * workspace: plb_attention_bwd_workspace_bytes() bytes, written and read by this call alone. Rows must be finite:
+ * a masked pair's probability is 0, and 0 times an infinity of the pair's other operand is NaN. The reference has
+ * no backward pass of its attention campaign. */
+size_t plb_attention_bwd_workspace_bytes(int batch, int seq, int q_heads);
+int plb_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* d_out, const float* lse,
+                      void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, int batch, int seq, int q_heads,
+                      int kv_heads, float scale, int window, float softcap, plb_status* status, void* stream);
+
+/* ------------------------------------------------------------------ RMS norm
+ * plb_rmsnorm_fwd: hidden = bf16(x + residual) (residual and hidden both given or both NULL; without them hidden is
+ * x), rstd f32 [rows] = 1 / sqrt(mean(hidden^2) + eps), y = bf16(hidden * rstd * weight) into y (bf16 [rows, width],
+ * may be NULL) and / or as MXFP8 into fp8 / sc (both or neither; width a multiple of 128; u8 [R, width] and
+ * [R / 128, width / 128, 32, 16] with R = rows up to a multiple of 128, rows past `rows` become zeros: the bytes of
+ * plb_mxfp8_quantize on y padded with zero rows). x and residual have row strides ld_* in elements (0 repeats a
+ * row), the outputs are contiguous. Any width and 2-byte alignment; 16-byte alignment throughout is faster. hidden
+ * may be residual or x itself (with equal layout), no other output may overlap an input.
+ * plb_rmsnorm_bwd: d_x = rstd * (g - n * mean(g * n)) + d_hidden with g = d_y * weight, n = hidden * rstd (the
+ * gradient of x and of residual alike; d_hidden, the gradient that reaches hidden past the norm, may be NULL);
+ * d_weight f32 [width] = sum over rows of d_y * n, in a fixed order. hidden is what the forward pass normalised.
+ * The reference normalises inside its decode megakernel only (campaigns/megakernel/host/mk_host_abi.h:35-85). */
+int plb_rmsnorm_fwd(const void* x, int64_t ld_x, const void* residual, int64_t ld_residual, const void* weight, int64_t rows,
+                    int64_t width, float eps, void* hidden, float* rstd, void* y, void* fp8, void* sc, void* stream);
+size_t plb_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t width);
+int plb_rmsnorm_bwd(const void* d_y, int64_t ld_d_y, const void* hidden, int64_t ld_hidden, const float* rstd,
+                    const void* weight, const void* d_hidden, int64_t ld_d_hidden, int64_t rows, int64_t width, void* d_x,
+                    float* d_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------ routing
+ * plb_route_topk: logits [tokens, experts] (fp32, or bf16 with logits_bf16; row stride ld_logits) -> experts_out i32
+ * and weights_out f32 [tokens, topk], in the order of the choice. score 0: softmax over the experts, 1: sigmoid.
+ * The choice goes by score + bias (f32 [experts], may be NULL), ties to the lowest index, compared as exactly as
+ * fp64 allows; weights are the scores without the bias, divided by their sum over the chosen with renormalize, times
+ * scale. groups > 1: experts are `groups` equal runs, a group's score is its best choice value, or the sum of its two
+ * best with group_top2, and only the topk_groups best groups take part. A logit of -inf masks an expert: chosen
+ * after every unmasked one of the kept groups, with weight 0; a token without any unmasked expert gets the lowest
+ * indices and weights 0. NaN ranks below every number and spreads as the formulas say; the experts named are
+ * always valid and distinct. experts <= 1024, topk <= 32, groups <= 32.
+ * plb_route_topk_bwd: gradient of the weights with respect to the logits (the logits' type), for the experts that
+ * were chosen; an expert that a token names twice counts twice, an index out of range not at all. The reference
+ * takes routes as inputs (campaigns/mok/host/mok_port_host.py:273-282 draws them with a top-k). */
+int plb_route_topk(const void* logits, int64_t ld_logits, int logits_bf16, const float* bias, int64_t tokens, int experts,
+                   int topk, int score, int groups, int topk_groups, int group_top2, int renormalize, float scale,
+                   int32_t* experts_out, float* weights_out, void* stream);
+int plb_route_topk_bwd(const float* d_weights, const void* logits, int64_t ld_logits, int logits_bf16, const int32_t* experts_in,
+                       int64_t tokens, int experts, int topk, int score, int renormalize, float scale, void* d_logits,
+                       void* stream);
+
 /* ------------------------------------------------------------------ linked images
  * Load and launch a linked pipeline image (`pipeline.cubin` + `link.json` of the link driver):
  * the roles of CudaBackend in the reference (pipec/src/pipec2/host/cuda.py:123-286: module load,

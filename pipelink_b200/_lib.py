@@ -108,6 +108,14 @@ PROTOTYPES = {
     "plb_attention_fwd_cp": (c_int, [c_void_p] * 6 + [c_int, c_int, c_int, c_int, ctypes.c_uint64, ctypes.c_uint64, c_float,
                                      c_void_p, ctypes.c_uint32, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_int,
                                      c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "plb_attention_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "plb_attention_bwd": (c_int, [c_void_p] * 10 + [c_size_t, c_int, c_int, c_int, c_int, c_float, c_int, c_float, c_void_p, c_void_p]),
+    "plb_rmsnorm_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_float] + [c_void_p] * 6),
+    "plb_rmsnorm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "plb_rmsnorm_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                                c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "plb_route_topk": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64] + [c_int] * 7 + [c_float, c_void_p, c_void_p, c_void_p]),
+    "plb_route_topk_bwd": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64] + [c_int] * 4 + [c_float, c_void_p, c_void_p]),
     "plb_image_load": (c_int, [c_void_p, c_char_p, c_int, POINTER(c_void_p), POINTER(c_void_p)]),
     "plb_image_launch": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
     "plb_image_launch_cooperative": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),

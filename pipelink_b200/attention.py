@@ -10,6 +10,8 @@ need them (``plb_cp_push_kv``) and bumps one readiness counter per 128-token blo
 kernel's load lane acquires a block's counter right before its first TMA of that block. A step is
 [group barrier] -> push -> attention, all on one stream: the push never waits on peers, so no two
 kernels on one GPU wait on each other.
+
+Training: ``attention_bwd(d_out, q, k, v, out, lse)`` gives the gradients of ``attention_fwd`` (single GPU).
 """
 from __future__ import annotations
 
@@ -21,7 +23,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .mok import DeviceStatus, _stream
+from .mok import DeviceStatus, _stream, dense, device_of
 
 BLK, D = 128, 128
 
@@ -81,11 +83,16 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, check: b
     """q [B, S, Hq, 128], k / v [B, S, Hkv, 128] bf16 CUDA. Returns (O like q, LSE f32 [B*Hq, S]).
     `pair_heads` None picks the two-heads-per-CTA kernel whenever Hq / Hkv is even. `window` > 0 adds
     the sliding-window mask (a query sees its last `window` keys), `softcap` > 0 the tanh soft cap
-    on the scaled scores; both are the reference's mask / score stage variants."""
+    on the scaled scores; both are the reference's mask / score stage variants. A sequence that is not a
+    multiple of 128 is run padded (the padding's keys lie behind every query's) and cut back."""
     B, S, Hq, d = q.shape
-    if d != D or S % BLK or q.dtype != torch.bfloat16:
-        raise ValueError("attention_fwd wants bf16, head_dim 128 and a sequence that is a multiple of 128")
+    if d != D or S < 1 or q.dtype != torch.bfloat16:
+        raise ValueError("attention_fwd wants bf16, head_dim 128 and a sequence of at least one token")
     Hkv = k.shape[2]
+    if S % BLK:
+        q, k, v = (torch.nn.functional.pad(t, (0, 0, 0, 0, 0, BLK - S % BLK)) for t in (q, k, v))
+        out, lse = attention_fwd(q, k, v, check=check, pair_heads=pair_heads, window=window, softcap=softcap)
+        return out[:, :S].contiguous(), lse[:, :S].contiguous()
     out = torch.empty_like(q)
     lse = torch.empty((B * Hq, S), dtype=torch.float32, device=q.device)
     step = heads_per_work(Hq, Hkv) if pair_heads is None else (2 if pair_heads else 1)
@@ -96,6 +103,44 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, check: b
     if check:
         status.check("attention_fwd")
     return out, lse
+
+
+def attention_bwd(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
+                  *, window: int = 0, softcap: float = 0.0, check: bool = True, status: DeviceStatus | None = None):
+    """Gradients of ``attention_fwd(q, k, v, window=, softcap=)``, whose results `out` and `lse` are passed back in with the
+    gradient of `out`: (dq, dk, dv), bf16 like q, k, v. Any sequence length; dk and dv are summed over the query heads of their
+    group. The same inputs give the same bits. `check` synchronises and raises on a device-side failure; under stream capture,
+    or in a loop that checks once, pass check=False and a `status` of your own."""
+    B, S, Hq, d = q.shape if q.dim() == 4 else (0, 0, 0, 0)
+    Hkv = k.shape[2] if k.dim() == 4 else 0
+    if d != D or k.shape != (B, S, Hkv, D) or v.shape != k.shape or out.shape != q.shape or d_out.shape != q.shape:
+        raise ValueError("attention_bwd wants q, out, d_out [B, S, Hq, 128] and k, v [B, S, Hkv, 128]")
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError("the query heads must be a multiple of the KV heads")
+    if lse.shape != (B * Hq, S) or lse.dtype != torch.float32:
+        raise ValueError("lse is f32 [B * Hq, S], as attention_fwd returns it")
+    for t in (d_out, q, k, v, out):
+        if t.dtype != torch.bfloat16 or not t.is_cuda or t.device != q.device:
+            raise ValueError("attention_bwd wants bf16 CUDA tensors on one device")
+    if lse.device != q.device:
+        raise ValueError("lse lies on another device")
+    if window < 0 or not softcap >= 0.0:
+        raise ValueError("window and softcap are 0 (off) or positive")
+    with device_of(q):
+        d_out, q, k, v, out, lse = (dense(t) for t in (d_out, q, k, v, out, lse))
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        if B == 0 or S == 0:
+            return dq, dk, dv
+        nbytes = _lib.load().plb_attention_bwd_workspace_bytes(B, S, Hq)
+        workspace = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
+        own = status is None
+        status = DeviceStatus(q.device) if own else status
+        _lib.call("plb_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), d_out.data_ptr(), lse.data_ptr(),
+                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(), nbytes, B, S, Hq, Hkv, 1.0 / math.sqrt(D),
+                  int(window), float(softcap), status.buf.data_ptr(), _stream())
+        if check:
+            status.check("attention_bwd")
+    return dq, dk, dv
 
 
 class CpRank:

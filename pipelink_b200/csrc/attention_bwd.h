@@ -1,0 +1,41 @@
+// Arguments of the attention backward kernels (attention_bwd.cu).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "common.cuh"
+
+namespace plb {
+
+struct AttnBwdParams {
+  const __nv_bfloat16* out;
+  const __nv_bfloat16* d_out;
+  const float* lse;          // [batch * q_heads, seq], natural log
+  float* lse2;               // [batch * q_heads, seq_pad]: base 2, +inf where a row has no probabilities
+  float* delta;              // [batch * q_heads, seq_pad]
+  __nv_bfloat16* dq;
+  __nv_bfloat16* dk;
+  __nv_bfloat16* dv;
+  int batch, seq, tiles, q_heads, kv_heads, group;
+  int64_t seq_pad;           // tiles * 128
+  int window;                // 0 = none
+  float scale, scale_log2;
+  float cap_in, cap_out;     // soft cap: y = cap_out * tanh in base 2, 2 log2(e) * scale / cap on the way in
+  Status* status;
+};
+
+struct AttnBwdArgs {
+  const void *q, *k, *v, *out, *d_out;
+  const float* lse;
+  void *dq, *dk, *dv;
+  float* workspace;          // 2 * batch * q_heads * (seq rounded up to 128) floats, 16-byte aligned
+  int batch, seq, q_heads, kv_heads;
+  float scale, softcap;
+  int window;
+  int num_sms;
+  Status* status;
+};
+
+cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream);
+
+}  // namespace plb

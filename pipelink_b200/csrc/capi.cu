@@ -5,6 +5,7 @@
 #include <string.h>
 
 #include "attention.h"
+#include "attention_bwd.h"
 #include "decode.h"
 #include "kernels.h"
 
@@ -1012,6 +1013,115 @@ int plb_tensor_map_2d_u32(void* out128, const void* base, uint64_t rows, uint64_
   if (rc != CUDA_SUCCESS) return PLB_E_BUILD;
   memcpy(out128, &map, sizeof(map));
   return PLB_OK;
+}
+
+size_t plb_attention_bwd_workspace_bytes(int batch, int seq, int q_heads) {
+  if (batch < 0 || seq < 0 || q_heads < 0) return 0;
+  return static_cast<size_t>(2) * batch * q_heads * ((static_cast<size_t>(seq) + 127) / 128 * 128) * sizeof(float);
+}
+
+int plb_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* d_out, const float* lse,
+                      void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, int batch, int seq, int q_heads,
+                      int kv_heads, float scale, int window, float softcap, plb_status* status, void* stream) {
+  if (batch < 0 || seq < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || window < 0 || !(softcap >= 0.0f))
+    return PLB_E_ARGUMENT;
+  if (batch == 0 || seq == 0) return PLB_OK;
+  if (!q || !k || !v || !out || !d_out || !lse || !dq || !dk || !dv || !workspace || !status) return PLB_E_ARGUMENT;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(d_out) || !aligned16(dq) ||
+      !aligned16(dk) || !aligned16(dv) || !aligned16(workspace))
+    return PLB_E_ARGUMENT;
+  if (workspace_bytes < plb_attention_bwd_workspace_bytes(batch, seq, q_heads)) return PLB_E_CAPACITY;
+  // tiles and work items are counted in 32 bits
+  if (seq > (1 << 30) || (static_cast<int64_t>(seq) + 127) / 128 * batch * q_heads > (1 << 30)) return PLB_E_ARGUMENT;
+  plb::AttnBwdArgs a;
+  a.q = q; a.k = k; a.v = v; a.out = out; a.d_out = d_out; a.lse = lse;
+  a.dq = dq; a.dk = dk; a.dv = dv;
+  a.workspace = static_cast<float*>(workspace);
+  a.batch = batch; a.seq = seq; a.q_heads = q_heads; a.kv_heads = kv_heads;
+  a.scale = scale; a.window = window; a.softcap = softcap;
+  a.num_sms = sm_count();
+  a.status = reinterpret_cast<plb::Status*>(status);
+  if (a.num_sms <= 0) return PLB_E_CUDA;
+  return from_cuda(plb::launch_attention_bwd(a, static_cast<cudaStream_t>(stream)));
+}
+
+int plb_rmsnorm_fwd(const void* x, int64_t ld_x, const void* residual, int64_t ld_residual, const void* weight, int64_t rows,
+                    int64_t width, float eps, void* hidden, float* rstd, void* y, void* fp8, void* sc, void* stream) {
+  if (rows < 0 || width < 1 || rows > 0x7FFFFF00ll || width > 0x7FFFFFFFll || ld_x < 0 || ld_residual < 0 || !(eps >= 0.0f))
+    return PLB_E_ARGUMENT;
+  if (rows == 0) return PLB_OK;
+  if (!weight || (fp8 == nullptr) != (sc == nullptr) || (fp8 != nullptr && width % 128) || (!y && !fp8)) return PLB_E_ARGUMENT;
+  if (!x || !rstd || (residual == nullptr) != (hidden == nullptr)) return PLB_E_ARGUMENT;
+  if (fp8 != nullptr && (!aligned16(fp8) || !aligned16(sc))) return PLB_E_ARGUMENT;
+  plb::NormFwdArgs a;
+  a.x = x; a.residual = residual; a.weight = weight;
+  a.ld_x = ld_x; a.ld_residual = ld_residual; a.rows = rows; a.width = width;
+  a.eps = eps;
+  a.hidden = hidden; a.rstd = rstd; a.y = y; a.fp8 = fp8; a.sc = sc;
+  a.num_sms = sm_count();
+  if (a.num_sms <= 0) return PLB_E_CUDA;
+  return from_cuda(plb::launch_rmsnorm_fwd(a, static_cast<cudaStream_t>(stream)));
+}
+
+size_t plb_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t width) {
+  if (rows < 0 || width < 0) return 0;
+  return static_cast<size_t>(plb::norm_bwd_strips(rows)) * width * sizeof(float);
+}
+
+int plb_rmsnorm_bwd(const void* d_y, int64_t ld_d_y, const void* hidden, int64_t ld_hidden, const float* rstd,
+                    const void* weight, const void* d_hidden, int64_t ld_d_hidden, int64_t rows, int64_t width, void* d_x,
+                    float* d_weight, void* workspace, size_t workspace_bytes, void* stream) {
+  if (rows < 0 || width < 1 || rows > 0x7FFFFF00ll || width > 0x7FFFFFFFll || ld_d_y < 0 || ld_hidden < 0 || ld_d_hidden < 0)
+    return PLB_E_ARGUMENT;
+  if (!weight || !d_weight || !workspace) return PLB_E_ARGUMENT;
+  if (rows > 0 && (!d_y || !hidden || !rstd || !d_x)) return PLB_E_ARGUMENT;
+  if (workspace_bytes < plb_rmsnorm_bwd_workspace_bytes(rows, width)) return PLB_E_CAPACITY;
+  plb::NormBwdArgs a;
+  a.d_y = d_y; a.hidden = hidden; a.rstd = rstd; a.weight = weight; a.d_hidden = d_hidden;
+  a.ld_d_y = ld_d_y; a.ld_hidden = ld_hidden; a.ld_d_hidden = ld_d_hidden; a.rows = rows; a.width = width;
+  a.d_x = d_x; a.d_weight = d_weight; a.workspace = static_cast<float*>(workspace);
+  a.num_sms = sm_count();
+  if (a.num_sms <= 0) return PLB_E_CUDA;
+  return from_cuda(plb::launch_rmsnorm_bwd(a, static_cast<cudaStream_t>(stream)));
+}
+
+static bool route_shape_ok(int64_t tokens, int64_t ld_logits, int experts, int topk, int score, float scale) {
+  return tokens >= 0 && tokens <= (1ll << 32) && ld_logits >= 0 && experts >= 1 && experts <= 1024 && topk >= 1 && topk <= 32 &&
+         topk <= experts && (score == 0 || score == 1) && scale == scale;
+}
+
+int plb_route_topk(const void* logits, int64_t ld_logits, int logits_bf16, const float* bias, int64_t tokens, int experts,
+                   int topk, int score, int groups, int topk_groups, int group_top2, int renormalize, float scale,
+                   int32_t* experts_out, float* weights_out, void* stream) {
+  if (!route_shape_ok(tokens, ld_logits, experts, topk, score, scale)) return PLB_E_ARGUMENT;
+  if (groups < 1 || groups > 32 || experts % groups || topk_groups < 1 || topk_groups > groups ||
+      topk > topk_groups * (experts / groups))
+    return PLB_E_ARGUMENT;
+  if (tokens == 0) return PLB_OK;
+  if (!logits || !experts_out || !weights_out) return PLB_E_ARGUMENT;
+  plb::RouteArgs a;
+  a.logits = logits; a.bias = bias; a.tokens = tokens; a.ld_logits = ld_logits;
+  a.experts = experts; a.topk = topk; a.groups = topk_groups == groups ? 1 : groups;   // all groups kept: none are told apart
+  a.topk_groups = topk_groups == groups ? 1 : topk_groups;
+  a.bf16 = logits_bf16 != 0; a.sigmoid = score == 1; a.group_top2 = group_top2 != 0; a.renormalize = renormalize != 0;
+  a.scale = scale;
+  a.experts_out = experts_out; a.weights_out = weights_out;
+  return from_cuda(plb::launch_route_topk(a, static_cast<cudaStream_t>(stream)));
+}
+
+int plb_route_topk_bwd(const float* d_weights, const void* logits, int64_t ld_logits, int logits_bf16, const int32_t* experts_in,
+                       int64_t tokens, int experts, int topk, int score, int renormalize, float scale, void* d_logits,
+                       void* stream) {
+  if (!route_shape_ok(tokens, ld_logits, experts, topk, score, scale)) return PLB_E_ARGUMENT;
+  if (tokens == 0) return PLB_OK;
+  if (!d_weights || !logits || !experts_in || !d_logits) return PLB_E_ARGUMENT;
+  plb::RouteBwdArgs a;
+  a.d_weights = d_weights; a.logits = logits; a.experts_in = experts_in; a.tokens = tokens; a.ld_logits = ld_logits;
+  a.experts = experts; a.topk = topk;
+  a.bf16 = logits_bf16 != 0; a.sigmoid = score == 1; a.renormalize = renormalize != 0;
+  a.scale = scale;
+  a.d_logits = d_logits;
+  return from_cuda(plb::launch_route_topk_bwd(a, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -165,4 +165,59 @@ cudaError_t launch_ep_pull_rows(const void* const* xq_peers, const void* const* 
                                 const int* num_rows_dev, int64_t capacity, int hidden,
                                 void* x_routed_fp8, void* x_routed_sc, cudaStream_t stream);
 
+// ---- RMS norm (norm.cu). Row strides (ld_*) are in elements.
+struct NormFwdArgs {
+  const void* x;
+  const void* residual;      // or null
+  const void* weight;
+  int64_t ld_x, ld_residual, rows, width;
+  float eps;
+  void* hidden;              // [rows, width] when residual is given
+  float* rstd;               // [rows]
+  void* y;                   // [rows, width] or null
+  void* fp8;                 // [rows up to a multiple of 128, width] and its scales, or null
+  void* sc;
+  int num_sms;
+};
+struct NormBwdArgs {
+  const void* d_y;
+  const void* hidden;
+  const float* rstd;
+  const void* weight;
+  const void* d_hidden;      // or null
+  int64_t ld_d_y, ld_hidden, ld_d_hidden, rows, width;
+  void* d_x;                 // [rows, width]
+  float* d_weight;           // [width]
+  float* workspace;          // [norm_bwd_strips(rows), width]
+  int num_sms;
+};
+constexpr int kNormMaxStrips = 256;
+int64_t norm_bwd_strips(int64_t rows);
+cudaError_t launch_rmsnorm_fwd(const NormFwdArgs& a, cudaStream_t stream);
+cudaError_t launch_rmsnorm_bwd(const NormBwdArgs& a, cudaStream_t stream);
+
+// ---- routing (router.cu)
+struct RouteArgs {
+  const void* logits;        // [tokens, experts] fp32 or bf16, row stride ld_logits
+  const float* bias;         // [experts] or null
+  int64_t tokens, ld_logits;
+  int experts, topk, groups, topk_groups;
+  bool bf16, sigmoid, group_top2, renormalize;
+  float scale;
+  int* experts_out;          // [tokens, topk]
+  float* weights_out;
+};
+struct RouteBwdArgs {
+  const float* d_weights;    // [tokens, topk]
+  const void* logits;
+  const int* experts_in;     // [tokens, topk]
+  int64_t tokens, ld_logits;
+  int experts, topk;
+  bool bf16, sigmoid, renormalize;
+  float scale;
+  void* d_logits;            // [tokens, experts], the logits' type
+};
+cudaError_t launch_route_topk(const RouteArgs& a, cudaStream_t stream);
+cudaError_t launch_route_topk_bwd(const RouteBwdArgs& a, cudaStream_t stream);
+
 }  // namespace plb

@@ -8,6 +8,7 @@ goes through the C ABI in ``include/pipelink_b200.h``; torch only owns the memor
 """
 from __future__ import annotations
 
+import contextlib
 from dataclasses import dataclass
 
 import torch
@@ -47,6 +48,26 @@ def _ptr(t):
 
 def _stream():
     return torch.cuda.current_stream().cuda_stream
+
+
+def device_of(t: torch.Tensor):
+    """Context in which launches go to the tensor's device (its current stream there)."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def dense(t: torch.Tensor) -> torch.Tensor:
+    """The tensor itself where it is contiguous and starts on 16 bytes, a copy otherwise."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def rows_of(t: torch.Tensor):
+    """[..., width] as 2-D rows of unit-stride elements and their stride: a view where one exists (a slice of a wider
+    tensor, a broadcast row), a copy otherwise."""
+    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
 
 
 def schedule_capacity(tokens_total: int, num_local_experts: int, padding: int | None = None) -> int:
