@@ -191,7 +191,7 @@ struct NormBwdArgs {
   float* workspace;          // [norm_bwd_strips(rows), width]
   int num_sms;
 };
-constexpr int kNormMaxStrips = 256;
+constexpr int kNormMaxStrips = 512;
 int64_t norm_bwd_strips(int64_t rows);
 cudaError_t launch_rmsnorm_fwd(const NormFwdArgs& a, cudaStream_t stream);
 cudaError_t launch_rmsnorm_bwd(const NormBwdArgs& a, cudaStream_t stream);

@@ -6,6 +6,12 @@
 // What is normalised is h as it is stored, so the backward pass sees the numbers the forward pass used. Sums and
 // the statistics are fp32; y is rounded to bf16 before it is quantised, so the bytes are those of
 // plb_mxfp8_quantize on y.
+//
+// Both directions are bound by memory: a row is read once into registers, reduced by the TPR threads that hold it
+// and written from there. VEC is the elements a thread moves at a time: 8 (16 bytes) where width, strides and
+// addresses allow, else 1. Rows too wide for registers (16384 elements, 8192 unaligned) are read twice.
+#include <type_traits>
+
 #include "kernels.h"
 #include "mxfp8.cuh"
 
@@ -33,13 +39,255 @@ __device__ __forceinline__ float block_sum(float v) {
   return s;
 }
 __device__ __forceinline__ float round_bf16(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
 
-// One CTA per row, any width and alignment: the row is read twice, the second time from the cache.
+// VEC bf16 numbers as they travel.
+template <int VEC>
+struct Chunk;
+template <>
+struct Chunk<8> {
+  uint4 raw;
+  __device__ __forceinline__ void load(const void* base, int64_t i) { raw = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + i); }
+  __device__ __forceinline__ void store(void* base, int64_t i) const { *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(base) + i) = raw; }
+  __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ float get(int i) const {
+    const uint32_t w = i < 2 ? raw.x : i < 4 ? raw.y : i < 6 ? raw.z : raw.w;
+    return i & 1 ? bf16_hi(w) : bf16_lo(w);
+  }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+    raw = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+  }
+};
+template <>
+struct Chunk<1> {
+  __nv_bfloat16 raw;
+  __device__ __forceinline__ void load(const void* base, int64_t i) { raw = static_cast<const __nv_bfloat16*>(base)[i]; }
+  __device__ __forceinline__ void store(void* base, int64_t i) const { static_cast<__nv_bfloat16*>(base)[i] = raw; }
+  __device__ __forceinline__ void zero() { raw = __float2bfloat16_rn(0.0f); }
+  __device__ __forceinline__ float get(int) const { return __bfloat162float(raw); }
+  __device__ __forceinline__ void set(const float (&f)[1]) { raw = __float2bfloat16_rn(f[0]); }
+};
+
+// CTAs hold whole rows: several where a warp has a row to itself, one otherwise.
+template <int TPR>
+struct RowTeam {
+  static constexpr int kThreads = TPR < kNormThreads ? kNormThreads : TPR;
+  static constexpr int kRows = kThreads / TPR;
+  // Sum over a row's threads, the same bits in each; `round` alternates the buffers of consecutive sums.
+  __device__ static __forceinline__ float sum(float v, int round) {
+    v = warp_sum(v);
+    if constexpr (TPR > 32) {
+      __shared__ float part[2][kThreads / 32];
+      if ((threadIdx.x & 31) == 0) part[round & 1][threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; ++i) v += part[round & 1][i];
+    }
+    return v;
+  }
+};
+
+template <int VEC, int TPR, int NV>
+__global__ void __launch_bounds__(RowTeam<TPR>::kThreads)
+rmsnorm_fwd_rows(const NormFwdArgs a) {
+  using Team = RowTeam<TPR>;
+  const int t = threadIdx.x % TPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * Team::kRows + threadIdx.x / TPR;
+  const bool live = row < a.rows;
+  const int64_t width = a.width;
+  Chunk<VEC> h[NV], w[NV];
+  float sq = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+    h[i].zero();
+    w[i].zero();
+    if (c < width) {
+      if (live) h[i].load(a.x, row * a.ld_x + c);
+      w[i].load(a.weight, c);
+    }
+  }
+  if (a.residual != nullptr && live) {
+    Chunk<VEC> r[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+      if (c < width) r[i].load(a.residual, row * a.ld_residual + c);
+      else r[i].zero();
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+      float f[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] = h[i].get(e) + r[i].get(e);
+      h[i].set(f);
+      if (c < width) h[i].store(a.hidden, row * width + c);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sq = fmaf(h[i].get(e), h[i].get(e), sq);
+  const float rstd = rsqrtf(Team::sum(sq, 0) / static_cast<float>(width) + a.eps);
+  if (live && t == 0) a.rstd[row] = rstd;
+  const bool quantise = a.fp8 != nullptr;
+  if (!live && !(quantise && row < (a.rows + 127) / 128 * 128)) return;     // MXFP8 rows up to a multiple of 128 are zeros
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+    const bool in = c < width;
+    if (i * TPR * VEC >= width) break;            // the same for every thread of the row
+    float f[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = h[i].get(e) * rstd * w[i].get(e);
+    Chunk<VEC> y;
+    y.set(f);
+    if (live && in && a.y != nullptr) y.store(a.y, row * width + c);
+    if (!quantise) continue;
+    // 32 / VEC adjacent lanes hold a block; width is a multiple of 128, so a block is wholly inside the row or outside
+    float amax = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      f[e] = live ? y.get(e) : 0.0f;
+      amax = fmaxf(amax, fabsf(f[e]));
+    }
+#pragma unroll
+    for (int o = 1; o < 32 / VEC; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+    const uint32_t s = e8m0_from_amax(amax);
+    const float inv = e8m0_inverse(s);
+    uint8_t* fp8 = static_cast<uint8_t*>(a.fp8) + row * width + c;
+    uint8_t* sc = static_cast<uint8_t*>(a.sc) + scale_offset(row, c >> 5, width >> 7);
+    if constexpr (VEC == 8) {
+      uint32_t word = s;                          // the four scales of 128 columns are one word
+      word |= __shfl_down_sync(0xFFFFFFFFu, s, 4) << 8;
+      word |= __shfl_down_sync(0xFFFFFFFFu, s, 8) << 16;
+      word |= __shfl_down_sync(0xFFFFFFFFu, s, 12) << 24;
+      if (in) {
+        *reinterpret_cast<uint2*>(fp8) = make_uint2(cvt_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                                                    cvt_e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+        if ((t & 15) == 0) *reinterpret_cast<uint32_t*>(sc) = word;
+      }
+    } else {
+      if (in) {
+        *fp8 = static_cast<uint8_t>(cvt_e4m3x4(f[0] * inv, 0.0f, 0.0f, 0.0f));
+        if ((t & 31) == 0) *sc = static_cast<uint8_t>(s);
+      }
+    }
+  }
+}
+
+// The gradient of x, and this CTA's share of the weight's: a thread keeps the sums of its columns over the rows
+// the CTA walks, so dy and h are read once for both.
+template <int VEC, int TPR, int NV>
+__global__ void __launch_bounds__(RowTeam<TPR>::kThreads)
+rmsnorm_bwd_rows(const NormBwdArgs a) {
+  using Team = RowTeam<TPR>;
+  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
+  const int64_t width = a.width, sets = (a.rows + Team::kRows - 1) / Team::kRows;
+  const float inv_width = 1.0f / static_cast<float>(width);
+  float dw[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) dw[i][e] = 0.0f;
+  // the weight's columns of this thread: kept in registers, or read again (from L1) where those are short
+  constexpr bool kKeepWeight = NV * VEC < 32;
+  Chunk<VEC> kept[kKeepWeight ? NV : 1];
+  auto weight = [&](int i) {
+    if constexpr (kKeepWeight) return kept[i];
+    const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+    Chunk<VEC> v;
+    v.zero();
+    if (c < width) v.load(a.weight, c);
+    return v;
+  };
+  if constexpr (kKeepWeight) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+      kept[i].zero();
+      if (c < width) kept[i].load(a.weight, c);
+    }
+  }
+  int round = 0;
+  for (int64_t set = blockIdx.x; set < sets; set += gridDim.x, ++round) {
+    const int64_t row = set * Team::kRows + team;
+    const bool live = row < a.rows;
+    Chunk<VEC> g[NV], h[NV], r[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+      g[i].zero();
+      h[i].zero();
+      r[i].zero();
+      if (live && c < width) {
+        g[i].load(a.d_y, row * a.ld_d_y + c);
+        h[i].load(a.hidden, row * a.ld_hidden + c);
+        if (a.d_hidden != nullptr) r[i].load(a.d_hidden, row * a.ld_d_hidden + c);
+      }
+    }
+    const float rstd = live ? a.rstd[row] : 0.0f;
+    float dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const Chunk<VEC> w = weight(i);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float n = h[i].get(e) * rstd;
+        dw[i][e] = fmaf(g[i].get(e), n, dw[i][e]);
+        dot = fmaf(g[i].get(e) * w.get(e), n, dot);
+      }
+    }
+    const float mean = Team::sum(dot, round) * inv_width;
+    if (!live) continue;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+      if (c >= width) continue;
+      const Chunk<VEC> w = weight(i);
+      float d[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        d[e] = fmaf(rstd, fmaf(-h[i].get(e) * rstd, mean, g[i].get(e) * w.get(e)), r[i].get(e));
+      Chunk<VEC> out;
+      out.set(d);
+      out.store(a.d_x, row * width + c);
+    }
+  }
+  if constexpr (Team::kRows > 1) {                 // the CTA's rows of each column, in their order
+    __shared__ float part[Team::kThreads][NV * VEC];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) part[threadIdx.x][i * VEC + e] = dw[i][e];
+    __syncthreads();
+    if (team != 0) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        for (int k = 1; k < Team::kRows; ++k) dw[i][e] += part[k * TPR + t][i * VEC + e];
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+    if (c >= width) continue;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) a.workspace[blockIdx.x * width + c + e] = dw[i][e];
+  }
+}
+
+// ---- any width: one CTA per row, the row read a second time from the cache
 __global__ void __launch_bounds__(kNormThreads)
-rmsnorm_fwd_kernel(const NormFwdArgs a) {
+rmsnorm_fwd_wide(const NormFwdArgs a) {
   const int64_t row = blockIdx.x;
   const int64_t width = a.width;
-  const bool live = row < a.rows;             // rows up to a multiple of 128 exist in the MXFP8 output only: zeros
+  const bool live = row < a.rows;
   const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(a.x) + row * a.ld_x;
   const __nv_bfloat16* r = a.residual ? static_cast<const __nv_bfloat16*>(a.residual) + row * a.ld_residual : nullptr;
   const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(a.weight);
@@ -73,7 +321,7 @@ rmsnorm_fwd_kernel(const NormFwdArgs a) {
 }
 
 __global__ void __launch_bounds__(kNormThreads)
-rmsnorm_bwd_kernel(const NormBwdArgs a) {
+rmsnorm_bwd_wide(const NormBwdArgs a) {
   const int64_t row = blockIdx.x;
   const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(a.d_y) + row * a.ld_d_y;
   const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(a.hidden) + row * a.ld_hidden;
@@ -93,7 +341,7 @@ rmsnorm_bwd_kernel(const NormBwdArgs a) {
 
 // Column sums of dy * n over one strip of rows: partial[strip][c].
 __global__ void __launch_bounds__(kNormThreads)
-rmsnorm_dw_kernel(const NormBwdArgs a, int64_t rows_per_strip) {
+rmsnorm_dw_wide(const NormBwdArgs a, int64_t rows_per_strip) {
   const int64_t c = static_cast<int64_t>(blockIdx.x) * kNormThreads + threadIdx.x;
   const int64_t r0 = blockIdx.y * rows_per_strip, r1 = r0 + rows_per_strip < a.rows ? r0 + rows_per_strip : a.rows;
   if (c >= a.width) return;
@@ -104,14 +352,53 @@ rmsnorm_dw_kernel(const NormBwdArgs a, int64_t rows_per_strip) {
   a.workspace[blockIdx.y * a.width + c] = s;
 }
 
-// d_weight = sum over the strips, in their order.
+// d_weight = sum over the strips: 32 columns a CTA, 8 strips at a time, the eight partial sums joined in their order.
 __global__ void __launch_bounds__(kNormThreads)
-rmsnorm_dw_sum_kernel(const float* __restrict__ partial, int strips, int64_t width, float* __restrict__ d_weight) {
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kNormThreads + threadIdx.x;
-  if (c >= width) return;
+rmsnorm_dw_sum(const float* __restrict__ partial, int strips, int64_t width, float* __restrict__ d_weight) {
+  __shared__ float part[kNormThreads / 32][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float s = 0.0f;
-  for (int i = 0; i < strips; ++i) s += partial[i * width + c];
+  if (c < width)
+#pragma unroll 4
+    for (int i = warp; i < strips; i += kNormThreads / 32) s += partial[i * width + c];
+  part[warp][lane] = s;
+  __syncthreads();
+  if (warp != 0 || c >= width) return;
+#pragma unroll
+  for (int i = 1; i < kNormThreads / 32; ++i) s += part[i][lane];
   d_weight[c] = s;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <int V, int T, int N>
+struct RowShape {
+  static constexpr int kVec = V, kTpr = T, kNv = N;
+};
+// Calls f with the row shape for a width, false where rows do not fit in registers. Rows that a warp can hold get a
+// warp, which needs no barrier; few wide rows get the largest team, as the time of one row is what counts then.
+template <class F>
+bool by_row_shape(bool vec, int64_t width, bool few, F&& f) {
+  if (vec) {
+    const int64_t n = width / 8;
+    if (n <= 32) f(RowShape<8, 32, 1>{});
+    else if (n <= 64) f(RowShape<8, 32, 2>{});
+    else if (n <= 128) f(RowShape<8, 32, 4>{});
+    else if (n <= 256) f(RowShape<8, 256, 1>{});
+    else if (few && n <= 512) f(RowShape<8, 512, 1>{});
+    else if (n <= 512) f(RowShape<8, 256, 2>{});
+    else if (n <= 1024) f(RowShape<8, 512, 2>{});
+    else if (n <= 2048) f(RowShape<8, 512, 4>{});
+    else return false;
+  } else {
+    if (width <= 128) f(RowShape<1, 32, 4>{});
+    else if (width <= 1024) f(RowShape<1, 256, 4>{});
+    else if (width <= 4096) f(RowShape<1, 256, 16>{});
+    else if (width <= 8192) f(RowShape<1, 512, 16>{});
+    else return false;
+  }
+  return true;
 }
 
 }  // namespace
@@ -121,22 +408,42 @@ int64_t norm_bwd_strips(int64_t rows) { return rows < kNormMaxStrips ? (rows > 0
 cudaError_t launch_rmsnorm_fwd(const NormFwdArgs& a, cudaStream_t stream) {
   const int64_t rows = a.fp8 != nullptr ? (a.rows + 127) / 128 * 128 : a.rows;
   if (rows == 0) return cudaSuccess;
-  rmsnorm_fwd_kernel<<<static_cast<unsigned>(rows), kNormThreads, 0, stream>>>(a);
+  const bool vec = a.width % 8 == 0 && a.ld_x % 8 == 0 && a.ld_residual % 8 == 0 && aligned16(a.x) && aligned16(a.residual) &&
+                   aligned16(a.weight) && aligned16(a.hidden) && aligned16(a.y);
+  const bool done = by_row_shape(vec, a.width, a.rows <= a.num_sms, [&](auto s) {
+    using S = decltype(s);
+    using Team = RowTeam<S::kTpr>;
+    rmsnorm_fwd_rows<S::kVec, S::kTpr, S::kNv><<<static_cast<unsigned>((rows + Team::kRows - 1) / Team::kRows), Team::kThreads, 0, stream>>>(a);
+  });
+  if (!done) rmsnorm_fwd_wide<<<static_cast<unsigned>(rows), kNormThreads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
 cudaError_t launch_rmsnorm_bwd(const NormBwdArgs& a, cudaStream_t stream) {
-  const int64_t strips = norm_bwd_strips(a.rows), per = (a.rows + strips - 1) / strips;
-  const unsigned columns = static_cast<unsigned>((a.width + kNormThreads - 1) / kNormThreads);
-  if (a.rows > 0) {
-    rmsnorm_bwd_kernel<<<static_cast<unsigned>(a.rows), kNormThreads, 0, stream>>>(a);
+  const bool vec = a.width % 8 == 0 && a.ld_d_y % 8 == 0 && a.ld_hidden % 8 == 0 && a.ld_d_hidden % 8 == 0 && aligned16(a.d_y) &&
+                   aligned16(a.hidden) && aligned16(a.d_hidden) && aligned16(a.weight) && aligned16(a.d_x);
+  int64_t strips = norm_bwd_strips(a.rows);
+  const bool done = by_row_shape(vec, a.width, a.rows <= a.num_sms, [&](auto s) {
+    using S = decltype(s);
+    using Team = RowTeam<S::kTpr>;
+    const int64_t sets = (a.rows + Team::kRows - 1) / Team::kRows;
+    const int64_t most = static_cast<int64_t>(a.num_sms) * (Team::kThreads > 256 ? 1 : 3);
+    strips = sets < 1 ? 1 : sets;
+    if (strips > most) strips = most;
+    if (strips > kNormMaxStrips) strips = kNormMaxStrips;
+    rmsnorm_bwd_rows<S::kVec, S::kTpr, S::kNv><<<static_cast<unsigned>(strips), Team::kThreads, 0, stream>>>(a);
+  });
+  if (!done) {
+    const int64_t per = (a.rows + strips - 1) / strips;
+    if (a.rows > 0) rmsnorm_bwd_wide<<<static_cast<unsigned>(a.rows), kNormThreads, 0, stream>>>(a);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
+    rmsnorm_dw_wide<<<dim3(static_cast<unsigned>((a.width + kNormThreads - 1) / kNormThreads), static_cast<unsigned>(strips)), kNormThreads, 0,
+                      stream>>>(a, per > 0 ? per : 1);
   }
-  rmsnorm_dw_kernel<<<dim3(columns, static_cast<unsigned>(strips)), kNormThreads, 0, stream>>>(a, per > 0 ? per : 1);
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
-  rmsnorm_dw_sum_kernel<<<columns, kNormThreads, 0, stream>>>(a.workspace, static_cast<int>(strips), a.width, a.d_weight);
+  rmsnorm_dw_sum<<<static_cast<unsigned>((a.width + 31) / 32), kNormThreads, 0, stream>>>(a.workspace, static_cast<int>(strips), a.width, a.d_weight);
   return cudaGetLastError();
 }
 

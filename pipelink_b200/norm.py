@@ -11,7 +11,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .mok import _ptr, _stream, device_of, rows_of
+from .mok import _ptr, _stream, dense, device_of, rows_of
 
 
 @dataclass(frozen=True)
@@ -50,7 +50,7 @@ def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
         rows = x.numel() // width
         x2, ld_x = rows_of(x)
         r2, ld_r = rows_of(residual) if residual is not None else (None, 0)
-        weight = weight.contiguous()
+        weight = dense(weight)
         dev, padded = x.device, (rows + 127) // 128 * 128
         if into is None:
             u8 = dict(dtype=torch.uint8, device=dev)
@@ -94,7 +94,7 @@ def rmsnorm_bwd(d_y: torch.Tensor, hidden: torch.Tensor, rstd: torch.Tensor, wei
         g2, ld_g = rows_of(d_y)
         h2, ld_h = rows_of(hidden)
         e2, ld_e = rows_of(d_hidden) if d_hidden is not None else (None, 0)
-        rstd, weight = rstd.contiguous(), weight.contiguous()
+        rstd, weight = rstd.contiguous(), dense(weight)
         d_x = torch.empty(hidden.shape, dtype=torch.bfloat16, device=hidden.device)
         d_weight = torch.empty(width, dtype=torch.float32, device=hidden.device)
         nbytes = _lib.load().plb_rmsnorm_bwd_workspace_bytes(rows, width)

@@ -76,7 +76,7 @@ def test_gradient_against_differences(native_lib):
 
 
 def test_strides_alignment_broadcast_and_shapes(native_lib):
-    from pipelink_b200 import norm
+    from pipelink_b200 import mok, norm
     rows, width = 37, 512
     x, r, w, dy = make(rows, width, seed=4)
     want = norm.rmsnorm_fwd(x, w, r, out="both")
@@ -86,7 +86,16 @@ def test_strides_alignment_broadcast_and_shapes(native_lib):
         wide[:, spread:spread + width] = r
         xs, rs = wide[:, first:first + width], wide[:, spread:spread + width]
         got = norm.rmsnorm_fwd(xs, w, rs, out="both")
-        assert all(torch.equal(getattr(got, f), getattr(want, f)) for f in ("hidden", "rstd", "y", "fp8", "sc"))
+        # off 16-byte boundaries other threads hold other columns, so the squares are summed in another order: two fp32
+        # sums of `width` positive terms differ by at most 2 (width + 8) 2^-24 of their value, rstd by half of that and
+        # its own rounding, and y by as much before both are rounded to bf16, half a step each
+        assert torch.equal(got.hidden, want.hidden)
+        assert ((got.rstd - want.rstd).abs() <= 2 * (width + 8) * F * want.rstd).all()
+        assert ((got.y.double() - want.y.double()).abs() <= 2 * (H + (width + 8) * F) * want.y.double().abs()).all()
+        padded = torch.zeros(128, width, dtype=torch.bfloat16, device="cuda")
+        padded[:rows] = got.y
+        q, sc, _, _ = mok.mxfp8_quantize(padded)
+        assert torch.equal(got.fp8, q) and torch.equal(got.sc, sc)
         a, b = norm.rmsnorm_bwd(xs, rs, want.rstd, w, xs), norm.rmsnorm_bwd(x, r, want.rstd, w, x)
         assert torch.allclose(a[1], b[1], rtol=0, atol=float(1e-4 * b[1].abs().max())) and \
             ((a[0].double() - b[0].double()).abs() <= 2 * H * b[0].double().abs() + 1e-6).all()
