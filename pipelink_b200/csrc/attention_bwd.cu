@@ -356,9 +356,9 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         const int lo = p.window > 0 ? q_pos - key0 - p.window + 1 : 0;
         const bool masked = __any_sync(kFullMask, hi < 64 || lo > 0);
         float pr[64];
+        uint32_t v[32], pk[32];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t v[32];
           tc_ld_32x32b_x32(s_addr + c * 32, v);
           tc_wait_ld();
 #pragma unroll
@@ -370,22 +370,24 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         }
         if (!warp_wait(BAR(dp_full), blk & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 421)) { ok = false; break; }
         tc_fence_after();
-        uint32_t pk[32];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t v[32];
           tc_ld_32x32b_x32(t_dp + lane_addr + half * 64 + c * 32, v);
           tc_wait_ld();
+          // one branch per tile: the tests of a masked tile cost as much as the arithmetic
+          if (masked) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int n = c * 32 + i;
-            float d = pr[n] * (__uint_as_float(v[i]) - delta);
-            if (masked && (n >= hi || n < lo)) d = 0.0f;
-            pr[n] = d;
+            for (int i = 0; i < 32; ++i) {
+              const int n = c * 32 + i;
+              pr[n] = n < hi && n >= lo ? pr[n] * (__uint_as_float(v[i]) - delta) : 0.0f;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) pr[c * 32 + i] *= __uint_as_float(v[i]) - delta;
           }
-        }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(pr[2 * i], pr[2 * i + 1]);
+          for (int i = 0; i < 16; ++i) pk[c * 16 + i] = pack_bf16(pr[c * 32 + 2 * i], pr[c * 32 + 2 * i + 1]);
+        }
         tc_st_32x32b_x32(s_addr, pk);
         tc_wait_st();
         tc_fence_before();
@@ -572,12 +574,8 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         if (!warp_wait(BAR(s_full), n & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 451)) { ok = false; break; }
         tc_fence_after();
         float pr[64];
-        uint32_t pk[32];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t v[32];
-          tc_ld_32x32b_x32(s_addr + c * 32, v);
-          tc_wait_ld();
+        uint32_t v[32], pk[32];
+        auto probabilities = [&](auto m, int c) {
 #pragma unroll
           for (int i4 = 0; i4 < 8; ++i4) {
             const float4 l = stat[c * 8 + i4];
@@ -588,12 +586,36 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
               const int q = c * 32 + i4 * 4 + e;
               float slope;
               float v1 = probability<kCap>(__uint_as_float(v[i4 * 4 + e]), ls[e], p, slope);
-              if (masked && (q < lo || q >= hi)) v1 = 0.0f;
+              if (decltype(m)::value && (q < lo || q >= hi)) v1 = 0.0f;
               if (e & 1) pk[q >> 1] = pack_bf16(last, v1);
               last = v1;
               pr[q] = kCap ? v1 * slope : v1;
             }
           }
+        };
+        auto gradients = [&](auto m, int c) {
+#pragma unroll
+          for (int i4 = 0; i4 < 8; ++i4) {
+            const float4 l = stat[32 + c * 8 + i4];
+            const float dl[4] = {l.x, l.y, l.z, l.w};
+            float last = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int q = c * 32 + i4 * 4 + e;
+              float d = pr[q] * (__uint_as_float(v[i4 * 4 + e]) - dl[e]);
+              if (decltype(m)::value && (q < lo || q >= hi)) d = 0.0f;
+              if (e & 1) pk[q >> 1] = pack_bf16(last, d);
+              last = d;
+            }
+          }
+        };
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          tc_ld_32x32b_x32(s_addr + c * 32, v);
+          tc_wait_ld();
+          // one branch per tile: the tests of a masked tile cost as much as the arithmetic
+          if (masked) probabilities(TrueTag{}, c);
+          else probabilities(FalseTag{}, c);
         }
         tc_st_32x32b_x32(s_addr, pk);
         tc_wait_st();
@@ -603,24 +625,11 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t v[32];
           tc_ld_32x32b_x32(dp_addr + c * 32, v);
           tc_wait_ld();
-#pragma unroll
-          for (int i4 = 0; i4 < 8; ++i4) {
-            const float4 l = stat[32 + c * 8 + i4];
-            const float dl[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int q = c * 32 + i4 * 4 + e;
-              float d = pr[q] * (__uint_as_float(v[i4 * 4 + e]) - dl[e]);
-              if (masked && (q < lo || q >= hi)) d = 0.0f;
-              pr[q] = d;
-            }
-          }
+          if (masked) gradients(TrueTag{}, c);
+          else gradients(FalseTag{}, c);
         }
-#pragma unroll
-        for (int e = 0; e < 32; ++e) pk[e] = pack_bf16(pr[2 * e], pr[2 * e + 1]);
         tc_st_32x32b_x32(dp_addr, pk);
         tc_wait_st();
         tc_fence_before();
