@@ -545,10 +545,11 @@ int plb_tp_gemm_bf16(const void* a_bf16, const void* b_bf16, const int32_t* bloc
  * the forward call wrote it. All contiguous and 16-byte aligned; any seq >= 1 (rows past a sequence's end are
  * neither read as keys nor written). The probabilities are recomputed from lse; dk and dv are summed over the
  * query heads of their group in fp32 and rounded once, with no atomics: the same inputs give the same bits.
- * workspace: plb_attention_bwd_workspace_bytes() bytes, written and read by this call alone. Rows must be finite:
+ * workspace: plb_attention_bwd_workspace_bytes() bytes, written and read by this call alone (its contents before and
+ * after mean nothing). status may be NULL: a bounded wait that runs out then goes unreported. Rows must be finite:
  * a masked pair's probability is 0, and 0 times an infinity of the pair's other operand is NaN. The reference has
  * no backward pass of its attention campaign. */
-size_t plb_attention_bwd_workspace_bytes(int batch, int seq, int q_heads);
+size_t plb_attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv_heads, int window);
 int plb_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* d_out, const float* lse,
                       void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, int batch, int seq, int q_heads,
                       int kv_heads, float scale, int window, float softcap, plb_status* status, void* stream);

@@ -108,7 +108,7 @@ PROTOTYPES = {
     "plb_attention_fwd_cp": (c_int, [c_void_p] * 6 + [c_int, c_int, c_int, c_int, ctypes.c_uint64, ctypes.c_uint64, c_float,
                                      c_void_p, ctypes.c_uint32, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_int,
                                      c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
-    "plb_attention_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "plb_attention_bwd_workspace_bytes": (c_size_t, [c_int] * 5),
     "plb_attention_bwd": (c_int, [c_void_p] * 10 + [c_size_t, c_int, c_int, c_int, c_int, c_float, c_int, c_float, c_void_p, c_void_p]),
     "plb_rmsnorm_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_float] + [c_void_p] * 6),
     "plb_rmsnorm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64]),

@@ -131,13 +131,13 @@ def attention_bwd(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         if B == 0 or S == 0:
             return dq, dk, dv
-        nbytes = _lib.load().plb_attention_bwd_workspace_bytes(B, S, Hq)
+        nbytes = _lib.load().plb_attention_bwd_workspace_bytes(B, S, Hq, Hkv, int(window))
         workspace = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
-        own = status is None
-        status = DeviceStatus(q.device) if own else status
+        if status is None and check:
+            status = DeviceStatus(q.device)
         _lib.call("plb_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), d_out.data_ptr(), lse.data_ptr(),
                   dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(), nbytes, B, S, Hq, Hkv, 1.0 / math.sqrt(D),
-                  int(window), float(softcap), status.buf.data_ptr(), _stream())
+                  int(window), float(softcap), 0 if status is None else status.buf.data_ptr(), _stream())
         if check:
             status.check("attention_bwd")
     return dq, dk, dv

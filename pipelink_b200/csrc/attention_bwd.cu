@@ -32,9 +32,10 @@ using namespace attn;
 namespace {
 
 constexpr int kBwdThreads = 384;      // warp 0 TMA, warp 1 MMA, warps 4-11 compute
-constexpr int kCompute = 256;
+constexpr int kComputeWarps = 8;
 constexpr uint32_t kFullMask = 0xFFFFFFFFu;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kBwdRuns = 148;         // runs of steps: a CTA on every SM; no run waits for another, so fewer SMs only take longer
 
 // ---- shared-memory maps (offsets from a 1024-byte aligned base)
 constexpr int kDqK = 2 * kTileBytes, kDqKStages = 3;                  // after Q and dO
@@ -52,7 +53,7 @@ static_assert(kDqSmem <= 232448 && kKvSmem <= 232448, "227 KB of shared memory p
 
 struct DqBars {
   uint64_t q_full, q_empty, k_full[kDqKStages], k_empty[kDqKStages], v_full[kDqVStages], v_empty[kDqVStages];
-  uint64_t s_full[2], dp_full, ds_full, dq_full, dq_free, red, drain;
+  uint64_t s_full[2], dp_full, dp_read, ds_full, dq_full, dq_free, red, drain;
   uint32_t tmem_base, pad;
 };
 struct KvBars {
@@ -81,6 +82,11 @@ __device__ __forceinline__ DqItem dq_item(const AttnBwdParams& p, int w) {
   t.blocks = qb + 1 - t.first;
   return t;
 }
+// Query tiles that see key tile kb.
+__host__ __device__ __forceinline__ int kv_query_tiles(int tiles, int window, int kb) {
+  const int64_t last = window > 0 ? (static_cast<int64_t>(kb) * kBlk + kBlk - 1 + window - 1) / kBlk : tiles;
+  return (last < tiles - 1 ? static_cast<int>(last) : tiles - 1) + 1 - kb;
+}
 struct KvItem { int b, h, k0, first, tiles, n; };
 __device__ __forceinline__ KvItem kv_item(const AttnBwdParams& p, int w) {
   const int bh = p.batch * p.kv_heads;
@@ -90,16 +96,74 @@ __device__ __forceinline__ KvItem kv_item(const AttnBwdParams& p, int w) {
   t.h = r - t.b * p.kv_heads;
   t.k0 = kb * kBlk;
   t.first = kb;
-  int last = p.tiles - 1;
-  if (p.window > 0) last = min(static_cast<int64_t>(last), (static_cast<int64_t>(t.k0) + kBlk - 1 + p.window - 1) / kBlk);
-  t.tiles = last + 1 - kb;
+  t.tiles = kv_query_tiles(p.tiles, p.window, kb);
   t.n = t.tiles * p.group;
   return t;
 }
+// The key tiles' steps (a step: one query tile of one head) in one line, heaviest tiles first, cut into p.parts equal
+// runs: where run r begins, as a tile and a step of it.
+__device__ __forceinline__ int64_t run_begin(const AttnBwdParams& p, int r) { return p.steps * r / p.parts; }
+__device__ __forceinline__ void locate(const AttnBwdParams& p, int64_t at, int& w, int& step) {
+  const int bh = p.batch * p.kv_heads;
+  for (int kb = 0;; ++kb) {
+    const int n = kv_query_tiles(p.tiles, p.window, kb) * p.group;
+    if (at < static_cast<int64_t>(n) * bh || kb == p.tiles - 1) {
+      const int r = static_cast<int>(at / n);
+      w = kb * bh + r;
+      step = static_cast<int>(at - static_cast<int64_t>(r) * n);
+      return;
+    }
+    at -= static_cast<int64_t>(n) * bh;
+  }
+}
+// What a CTA works through: whole tiles (parts 0, the list walked forth and back) or its run, steps [i0, i1) of tile w.
+struct KvWalk {
+  int w, i0, i1, wave;
+  int64_t left;
+  KvItem t;
+  __device__ __forceinline__ bool begin(const AttnBwdParams& p, int items) {
+    wave = 0;
+    left = 0;
+    i0 = 0;
+    if (p.parts > 0) {
+      left = run_begin(p, blockIdx.x + 1) - run_begin(p, blockIdx.x);
+      locate(p, run_begin(p, blockIdx.x), w, i0);
+      if (left <= 0) return false;
+    } else {
+      w = snake(0);
+      if (w >= items) return false;
+    }
+    set(p);
+    return true;
+  }
+  __device__ __forceinline__ bool next(const AttnBwdParams& p, int items) {
+    if (p.parts > 0) {
+      left -= i1 - i0;
+      if (left <= 0) return false;
+      ++w;
+      i0 = 0;
+    } else {
+      w = snake(++wave);
+      if (w >= items) return false;      // only the last wave is short
+    }
+    set(p);
+    return true;
+  }
+  __device__ __forceinline__ void set(const AttnBwdParams& p) {
+    t = kv_item(p, w);
+    i1 = p.parts > 0 && left < t.n - i0 ? i0 + static_cast<int>(left) : t.n;
+  }
+};
 
 // A role's wait: the warp's lanes agree on the outcome.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, Status* st, int code, int what) {
   return __all_sync(kFullMask, mbar_wait(bar, parity, st, code, what)) != 0;
+}
+// A compute warp's arrival: one for its 32 lanes (32 arrivals on one barrier are 32 shared-memory atomics in a row,
+// and with two barriers a tile those took a quarter of the compute warps' time).
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 __device__ __forceinline__ void warp_commit(uint32_t bar) {
   if (elect_one_sync()) tc_commit(bar);
@@ -149,16 +213,61 @@ __device__ __forceinline__ void linger() {   // copies in flight land before the
   }
 }
 
-// Base-2 exponent of a raw score and, with a cap, the cap's slope. tanh from exp2 and a division rather than
-// tanh.approx: the slope and the exponent both see its error, scaled by the cap.
+// Two fp32 lanes of one register pair: Blackwell's packed arithmetic takes one issue slot for both.
+struct Pair { uint64_t v; };
+__device__ __forceinline__ Pair make_pair(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ Pair make_pair(uint32_t a, uint32_t b) { return make_pair(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ void split(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair exp2_pair(Pair x) {
+  float a, b;
+  split(x, a, b);
+  return make_pair(ex2_approx(a), ex2_approx(b));
+}
+
+// Probabilities of two raw scores; with a cap also its slope. tanh from exp2 and a division rather than tanh.approx:
+// the slope and the exponent both see its error, scaled by the cap. minus_lse2: the rows' negated base-2 log-sum-exp.
 template <bool kCap>
-__device__ __forceinline__ float probability(float s, float lse2, const AttnBwdParams& p, float& slope) {
+__device__ __forceinline__ Pair probability(Pair s, Pair minus_lse2, const AttnBwdParams& p, Pair& slope) {
   if (kCap) {
-    const float t = 1.0f - __fdividef(2.0f, 1.0f + ex2_approx(fminf(s * p.cap_in, 60.0f)));   // tanh(x) = 1 - 2 / (1 + 2^(2 x log2 e))
-    slope = fmaf(-t, t, 1.0f);
-    return ex2_approx(fmaf(t, p.cap_out, -lse2));
+    float a, b;
+    split(mul2(s, make_pair(p.cap_in, p.cap_in)), a, b);
+    const Pair t = make_pair(1.0f - __fdividef(2.0f, 1.0f + ex2_approx(fminf(a, 60.0f))),    // tanh(x) = 1 - 2 / (1 + 2^(2 x log2 e))
+                             1.0f - __fdividef(2.0f, 1.0f + ex2_approx(fminf(b, 60.0f))));
+    slope = fma2(mul2(t, make_pair(-1.0f, -1.0f)), t, make_pair(1.0f, 1.0f));
+    return exp2_pair(fma2(t, make_pair(p.cap_out, p.cap_out), minus_lse2));
   }
-  return ex2_approx(fmaf(s, p.scale_log2, -lse2));
+  return exp2_pair(fma2(s, make_pair(p.scale_log2, p.scale_log2), minus_lse2));
+}
+__device__ __forceinline__ uint32_t pack_bf16(Pair p) {
+  float a, b;
+  split(p, a, b);
+  const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+// Zeroes a pair's members outside [lo, hi); i is the first one's index.
+__device__ __forceinline__ Pair keep_range(Pair p, int i, int lo, int hi) {
+  float a, b;
+  split(p, a, b);
+  return make_pair(i >= lo && i < hi ? a : 0.0f, i + 1 >= lo && i + 1 < hi ? b : 0.0f);
 }
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
@@ -180,12 +289,23 @@ __device__ __forceinline__ void store_half_row(const uint32_t (&a)[32], const ui
   }
 }
 
+// A part's slot: dV then dK, [32 column quadruples][128 rows].
+constexpr int kPartVecs = 2 * 32 * kBlk;
+__device__ __forceinline__ void store_part(const uint32_t (&a)[32], const uint32_t (&b)[32], float4* dst) {
+#pragma unroll
+  for (int g = 0; g < 16; ++g) {
+    const int i = (g & 7) * 4;
+    dst[g * kBlk] = g < 8 ? make_float4(__uint_as_float(a[i]), __uint_as_float(a[i + 1]), __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]))
+                          : make_float4(__uint_as_float(b[i]), __uint_as_float(b[i + 1]), __uint_as_float(b[i + 2]), __uint_as_float(b[i + 3]));
+  }
+}
+
 #define PLB_BAR(type, base, name) (sb + (base) + offsetof(type, name))
 
 // ------------------------------------------------------------------------------------------ dQ
 // TMEM columns: dQ 0-127, S 128-255 and 256-383 (two buffers), dP 384-511. dX overwrites the S buffer it came
-// from, as the A operand of dQ += dX K. Issue order: S(j+1), dQ(j), dP(j+1); S(j+1) runs while the compute warps
-// finish dX(j), dQ(j) and dP(j+1) while they exponentiate S(j+1).
+// from, as the A operand of dQ += dX K. dP(j+1) is issued as soon as dP(j) has been read into registers, S(j+2) as
+// soon as dQ(j) has released its buffer, so the compute warps find their next operands ready.
 template <bool kCap>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
@@ -208,10 +328,11 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     mbar_init(BAR(s_full), 1);
     mbar_init(BAR(s_full) + 8, 1);
     mbar_init(BAR(dp_full), 1);
-    mbar_init(BAR(ds_full), kCompute);
+    mbar_init(BAR(dp_read), kComputeWarps);
+    mbar_init(BAR(ds_full), kComputeWarps);
     mbar_init(BAR(dq_full), 1);
-    mbar_init(BAR(dq_free), kCompute);
-    mbar_init(BAR(red), kCompute);
+    mbar_init(BAR(dq_free), kComputeWarps);
+    mbar_init(BAR(red), kComputeWarps);
     mbar_init(BAR(drain), 1);
     fence_mbar_init();
     prefetch_tensormap(&map_q);
@@ -288,19 +409,20 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       const int n = __shfl_sync(kFullMask, dq_item(p, w).blocks, 0);
       if (!warp_wait(BAR(q_full), it & 1u, p.status, ST_TIMEOUT_FULL, 412)) { ok = false; break; }
       tc_fence_after();
-      if (!issue_s(blk) || !issue_dp(blk)) { ok = false; break; }
+      if (!issue_s(blk) || !issue_dp(blk) || (n > 1 && !issue_s(blk + 1))) { ok = false; break; }
+      if (n == 1) warp_commit(BAR(q_empty));
       for (int j = 0; j < n && ok; ++j, ++blk) {
-        const bool more = j + 1 < n;
-        if (more && !issue_s(blk + 1)) { ok = false; break; }
+        if (!warp_wait(BAR(dp_read), blk & 1u, p.status, ST_TIMEOUT_FULL, 415)) { ok = false; break; }
+        if (j + 1 < n && !issue_dp(blk + 1)) { ok = false; break; }
+        if (j + 2 == n) warp_commit(BAR(q_empty));       // the last products that read Q and dO are issued: both may be replaced
         if (!warp_wait(BAR(ds_full), blk & 1u, p.status, ST_TIMEOUT_FULL, 413)) { ok = false; break; }
         if (j == 0 && !warp_wait(BAR(dq_free), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_TMEM_EMPTY, 414)) { ok = false; break; }
         tc_fence_after();
         const uint32_t ks = blk % kDqKStages;
         mma_from_tmem(t_dq, t_s + (blk & 1u) * 128, sb + kDqK + ks * kTileBytes, j != 0, BAR(k_empty) + 8 * ks);
-        if (more && !issue_dp(blk + 1)) { ok = false; break; }
+        if (j + 2 < n && !issue_s(blk + 2)) { ok = false; break; }
       }
       if (!ok) break;
-      warp_commit(BAR(q_empty));
       warp_commit(BAR(dq_full));
       ++it;
     }
@@ -311,89 +433,100 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     float* red = reinterpret_cast<float*>(smem + kDqRed);
     uint32_t it = 0, blk = 0;
     bool ok = true;
-    for (int wave = 0; ok && wave * static_cast<int>(gridDim.x) < items; ++wave) {
-      const int w = snake(wave);
-      if (w >= items) continue;
-      const DqItem t = dq_item(p, w);
+    // a tile's row in O, dO and dQ, and its half of delta and log-sum-exp: fetched for the next tile before this
+    // one's last product has been waited for
+    struct Row { int w; size_t at; float part, lse2; bool live; };
+    auto fetch = [&](int wave) {
+      Row r;
+      r.w = wave * static_cast<int>(gridDim.x) < items ? snake(wave) : items;
+      r.part = 0.0f;
+      r.lse2 = INFINITY;                         // rows past the end, and rows that saw no key, have no probabilities
+      r.live = false;
+      r.at = 0;
+      if (r.w >= items) return r;
+      const DqItem t = dq_item(p, r.w);
       const int q_pos = t.q0 + row;
-      const bool live = q_pos < p.seq;
-      const int64_t bh = static_cast<int64_t>(t.b) * p.q_heads + t.h;
-      const size_t at = ((static_cast<size_t>(t.b) * p.seq + (live ? q_pos : 0)) * p.q_heads + t.h) * kD + half * 64;
-      // delta: each thread half of its row, the two halves exchanged through shared memory
-      float part = 0.0f;
-      if (live) {
-        const uint4* o = reinterpret_cast<const uint4*>(p.out + at);
-        const uint4* g = reinterpret_cast<const uint4*>(p.d_out + at);
+      r.live = q_pos < p.seq;
+      if (!r.live) return r;
+      r.at = ((static_cast<size_t>(t.b) * p.seq + q_pos) * p.q_heads + t.h) * kD + half * 64;
+      const float l = p.lse[(static_cast<int64_t>(t.b) * p.q_heads + t.h) * p.seq + q_pos];
+      if (l > -INFINITY) r.lse2 = l * kLog2e;
+      const uint4* o = reinterpret_cast<const uint4*>(p.out + r.at);
+      const uint4* g = reinterpret_cast<const uint4*>(p.d_out + r.at);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint4 a = o[i], c = g[i];
-          part = fmaf(bf16_lo(a.x), bf16_lo(c.x), part); part = fmaf(bf16_hi(a.x), bf16_hi(c.x), part);
-          part = fmaf(bf16_lo(a.y), bf16_lo(c.y), part); part = fmaf(bf16_hi(a.y), bf16_hi(c.y), part);
-          part = fmaf(bf16_lo(a.z), bf16_lo(c.z), part); part = fmaf(bf16_hi(a.z), bf16_hi(c.z), part);
-          part = fmaf(bf16_lo(a.w), bf16_lo(c.w), part); part = fmaf(bf16_hi(a.w), bf16_hi(c.w), part);
-        }
+      for (int i = 0; i < 8; ++i) {
+        const uint4 a = o[i], c = g[i];
+        r.part = fmaf(bf16_lo(a.x), bf16_lo(c.x), r.part); r.part = fmaf(bf16_hi(a.x), bf16_hi(c.x), r.part);
+        r.part = fmaf(bf16_lo(a.y), bf16_lo(c.y), r.part); r.part = fmaf(bf16_hi(a.y), bf16_hi(c.y), r.part);
+        r.part = fmaf(bf16_lo(a.z), bf16_lo(c.z), r.part); r.part = fmaf(bf16_hi(a.z), bf16_hi(c.z), r.part);
+        r.part = fmaf(bf16_lo(a.w), bf16_lo(c.w), r.part); r.part = fmaf(bf16_hi(a.w), bf16_hi(c.w), r.part);
       }
-      float* red_it = red + (it & 1u) * 256;     // two buffers: the barrier below orders reuse
-      red_it[half * kBlk + row] = part;
-      mbar_arrive(BAR(red));
+      return r;
+    };
+    Row next = fetch(0);
+    for (int wave = 0; ok && wave * static_cast<int>(gridDim.x) < items; ++wave) {
+      const Row r = next;
+      if (r.w >= items) break;                   // only the last wave is short
+      const DqItem t = dq_item(p, r.w);
+      const int q_pos = t.q0 + row;
+      // delta: the two halves of a row's sum exchanged through shared memory, two buffers so that the barrier orders reuse
+      float* red_it = red + (it & 1u) * 256;
+      red_it[half * kBlk + row] = r.part;
+      warp_arrive(BAR(red));
       if (!warp_wait(BAR(red), it & 1u, p.status, ST_TIMEOUT_FULL, 423)) { ok = false; break; }
       const float delta = red_it[row] + red_it[kBlk + row];
-      float lse2 = INFINITY;                     // rows past the end, and rows that saw no key, have no probabilities
-      if (live) {
-        const float l = p.lse[bh * p.seq + q_pos];
-        if (l > -INFINITY) lse2 = l * kLog2e;
-      }
       if (half == 0) {
-        p.lse2[bh * p.seq_pad + q_pos] = lse2;
-        p.delta[bh * p.seq_pad + q_pos] = delta;
+        const int64_t at = (static_cast<int64_t>(t.b) * p.q_heads + t.h) * p.seq_pad + q_pos;
+        p.lse2[at] = -r.lse2;
+        p.delta[at] = -delta;
       }
+      const Pair minus_lse2 = make_pair(-r.lse2, -r.lse2), minus_delta = make_pair(-delta, -delta);
       for (int j = 0; j < t.blocks; ++j, ++blk) {
         const int key0 = (t.first + j) * kBlk + half * 64;
         const uint32_t s_addr = t_s + (blk & 1u) * 128 + lane_addr + half * 64;
         if (!warp_wait(BAR(s_full) + 8 * (blk & 1u), (blk >> 1) & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 420)) { ok = false; break; }
         tc_fence_after();
-        const int hi = live ? q_pos - key0 + 1 : 0;      // visible keys of this row: [lo, hi) of the 64
+        const int hi = r.live ? q_pos - key0 + 1 : 0;      // visible keys of this row: [lo, hi) of the 64
         const int lo = p.window > 0 ? q_pos - key0 - p.window + 1 : 0;
         const bool masked = __any_sync(kFullMask, hi < 64 || lo > 0);
-        float pr[64];
-        uint32_t v[32], pk[32];
+        Pair pr[32];
+        uint32_t v[32], u[32], pk[32];
+        tc_ld_32x32b_x32(s_addr, v);
+        tc_ld_32x32b_x32(s_addr + 32, u);
+        tc_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          tc_ld_32x32b_x32(s_addr + c * 32, v);
-          tc_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float slope;
-            const float pi = probability<kCap>(__uint_as_float(v[i]), lse2, p, slope);
-            pr[c * 32 + i] = kCap ? pi * slope : pi;
-          }
+        for (int i = 0; i < 32; ++i) {
+          Pair slope;
+          pr[i] = probability<kCap>(i < 16 ? make_pair(v[(2 * i) & 31], v[(2 * i + 1) & 31]) : make_pair(u[(2 * i) & 31], u[(2 * i + 1) & 31]),
+                                    minus_lse2, p, slope);
+          if (kCap) pr[i] = mul2(pr[i], slope);
         }
         if (!warp_wait(BAR(dp_full), blk & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 421)) { ok = false; break; }
         tc_fence_after();
+        tc_ld_32x32b_x32(t_dp + lane_addr + half * 64, v);
+        tc_ld_32x32b_x32(t_dp + lane_addr + half * 64 + 32, u);
+        tc_wait_ld();
+        tc_fence_before();
+        warp_arrive(BAR(dp_read));
+        // one branch per tile: the tests of a masked tile cost as much as the arithmetic
+        auto gradients = [&](auto m) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          tc_ld_32x32b_x32(t_dp + lane_addr + half * 64 + c * 32, v);
-          tc_wait_ld();
-          // one branch per tile: the tests of a masked tile cost as much as the arithmetic
-          if (masked) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int n = c * 32 + i;
-              pr[n] = n < hi && n >= lo ? pr[n] * (__uint_as_float(v[i]) - delta) : 0.0f;
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) pr[c * 32 + i] *= __uint_as_float(v[i]) - delta;
+          for (int i = 0; i < 32; ++i) {
+            const Pair dp = i < 16 ? make_pair(v[(2 * i) & 31], v[(2 * i + 1) & 31]) : make_pair(u[(2 * i) & 31], u[(2 * i + 1) & 31]);
+            Pair d = mul2(pr[i], add2(dp, minus_delta));
+            if (decltype(m)::value) d = keep_range(d, 2 * i, lo, hi);
+            pk[i] = pack_bf16(d);
           }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pk[c * 16 + i] = pack_bf16(pr[c * 32 + 2 * i], pr[c * 32 + 2 * i + 1]);
-        }
+        };
+        if (masked) gradients(TrueTag{});
+        else gradients(FalseTag{});
         tc_st_32x32b_x32(s_addr, pk);
         tc_wait_st();
         tc_fence_before();
-        mbar_arrive(BAR(ds_full));
+        warp_arrive(BAR(ds_full));
       }
       if (!ok) break;
+      next = fetch(wave + 1);
       if (!warp_wait(BAR(dq_full), it & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 422)) { ok = false; break; }
       tc_fence_after();
       uint32_t a[32], b[32];
@@ -401,9 +534,9 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       tc_ld_32x32b_x32(t_dq + lane_addr + half * 64 + 32, b);
       tc_wait_ld();
       tc_fence_before();
-      mbar_arrive(BAR(dq_free));
+      warp_arrive(BAR(dq_free));
       ++it;
-      if (live) store_half_row(a, b, p.scale, p.dq + at);
+      if (r.live) store_half_row(a, b, p.scale, p.dq + r.at);
     }
   }
 #undef BAR
@@ -438,13 +571,13 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     mbar_init(BAR(kv_empty), 1);
     for (int s = 0; s < kKvQStages; ++s) { mbar_init(BAR(q_full) + 8 * s, 1); mbar_init(BAR(q_empty) + 8 * s, 1); }
     for (int s = 0; s < kKvDoStages; ++s) { mbar_init(BAR(do_full) + 8 * s, 1); mbar_init(BAR(do_empty) + 8 * s, 1); }
-    for (int s = 0; s < kKvStatStages; ++s) { mbar_init(BAR(stat_full) + 8 * s, 1); mbar_init(BAR(stat_empty) + 8 * s, kCompute / 32); }
+    for (int s = 0; s < kKvStatStages; ++s) { mbar_init(BAR(stat_full) + 8 * s, 1); mbar_init(BAR(stat_empty) + 8 * s, kComputeWarps); }
     mbar_init(BAR(s_full), 1);
-    mbar_init(BAR(p_full), kCompute);
+    mbar_init(BAR(p_full), kComputeWarps);
     mbar_init(BAR(dp_full), 1);
-    mbar_init(BAR(ds_full), kCompute);
+    mbar_init(BAR(ds_full), kComputeWarps);
     mbar_init(BAR(acc_full), 1);
-    mbar_init(BAR(acc_free), kCompute);
+    mbar_init(BAR(acc_free), kComputeWarps);
     mbar_init(BAR(drain), 1);
     fence_mbar_init();
     prefetch_tensormap(&map_q);
@@ -466,10 +599,9 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   if (warp == 0) {
     uint32_t it = 0, n = 0;
     bool ok = true;
-    for (int wave = 0; ok && wave * static_cast<int>(gridDim.x) < items; ++wave) {
-      const int w = snake(wave);
-      if (w >= items) continue;
-      const KvItem t = kv_item(p, w);
+    KvWalk walk;
+    for (bool go = walk.begin(p, items); go && ok; go = walk.next(p, items)) {
+      const KvItem& t = walk.t;
       if (!warp_wait(BAR(kv_empty), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_EMPTY, 430)) { ok = false; break; }
       if (elect_one_sync()) {
         mbar_arrive_expect_tx(BAR(kv_full), 2 * kTileBytes);
@@ -478,8 +610,8 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       }
       __syncwarp();
       ++it;
-      int g = 0, qt = 0;
-      for (int i = 0; i < t.n; ++i, ++n) {
+      int g = walk.i0 / t.tiles, qt = walk.i0 % t.tiles;
+      for (int i = walk.i0; i < walk.i1; ++i, ++n) {
         const int h = t.h * p.group + g, row = (t.first + qt) * kBlk;
         const uint32_t qs = n % kKvQStages, ds = n % kKvDoStages, ss = n % kKvStatStages;
         if (!warp_wait(BAR(q_empty) + 8 * qs, ((n / kKvQStages) & 1u) ^ 1u, p.status, ST_TIMEOUT_EMPTY, 431)) { ok = false; break; }
@@ -523,10 +655,9 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       mma_tiles(t_dp, sb + kTileBytes, sb + kKvDo + ds * kTileBytes, BAR(dp_full));
       return true;
     };
-    for (int wave = 0; ok && wave * static_cast<int>(gridDim.x) < items; ++wave) {
-      const int w = snake(wave);
-      if (w >= items) continue;
-      const int steps = __shfl_sync(kFullMask, kv_item(p, w).n, 0);
+    KvWalk walk;
+    for (bool go = walk.begin(p, items); go && ok; go = walk.next(p, items)) {
+      const int steps = __shfl_sync(kFullMask, walk.i1 - walk.i0, 0);
       if (!warp_wait(BAR(kv_full), it & 1u, p.status, ST_TIMEOUT_FULL, 442)) { ok = false; break; }
       tc_fence_after();
       if (!issue_s(n) || !issue_dp(n)) { ok = false; break; }
@@ -555,13 +686,12 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     const uint32_t s_addr = t_s + lane_addr + half * 64, dp_addr = t_dp + lane_addr + half * 64;
     uint32_t it = 0, n = 0;
     bool ok = true;
-    for (int wave = 0; ok && wave * static_cast<int>(gridDim.x) < items; ++wave) {
-      const int w = snake(wave);
-      if (w >= items) continue;
-      const KvItem t = kv_item(p, w);
+    KvWalk walk;
+    for (bool go = walk.begin(p, items); go && ok; go = walk.next(p, items)) {
+      const KvItem& t = walk.t;
       const int k_pos = t.k0 + row;
-      int qt = 0;
-      for (int i = 0; i < t.n; ++i, ++n) {
+      int qt = walk.i0 % t.tiles;
+      for (int i = walk.i0; i < walk.i1; ++i, ++n) {
         const int q0 = (t.first + qt) * kBlk + half * 64;
         if (++qt == t.tiles) qt = 0;
         const uint32_t ss = n % kKvStatStages;
@@ -573,86 +703,87 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         if (!warp_wait(BAR(stat_full) + 8 * ss, (n / kKvStatStages) & 1u, p.status, ST_TIMEOUT_FULL, 450)) { ok = false; break; }
         if (!warp_wait(BAR(s_full), n & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 451)) { ok = false; break; }
         tc_fence_after();
-        float pr[64];
-        uint32_t v[32], pk[32];
-        auto probabilities = [&](auto m, int c) {
+        Pair pr[32];
+        uint32_t v[32], u[32], pk[32];
+        // one branch per tile: the tests of a masked tile cost as much as the arithmetic
+        auto probabilities = [&](auto m) {
 #pragma unroll
-          for (int i4 = 0; i4 < 8; ++i4) {
-            const float4 l = stat[c * 8 + i4];
-            const float ls[4] = {l.x, l.y, l.z, l.w};
-            float last = 0.0f;
+          for (int i = 0; i < 32; i += 2) {
+            const float4 l = stat[i >> 1];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int q = c * 32 + i4 * 4 + e;
-              float slope;
-              float v1 = probability<kCap>(__uint_as_float(v[i4 * 4 + e]), ls[e], p, slope);
-              if (decltype(m)::value && (q < lo || q >= hi)) v1 = 0.0f;
-              if (e & 1) pk[q >> 1] = pack_bf16(last, v1);
-              last = v1;
-              pr[q] = kCap ? v1 * slope : v1;
+            for (int e = i; e < i + 2; ++e) {
+              Pair slope;
+              pr[e] = probability<kCap>(e < 16 ? make_pair(v[(2 * e) & 31], v[(2 * e + 1) & 31]) : make_pair(u[(2 * e) & 31], u[(2 * e + 1) & 31]),
+                                        e == i ? make_pair(l.x, l.y) : make_pair(l.z, l.w), p, slope);
+              if (decltype(m)::value) pr[e] = keep_range(pr[e], 2 * e, lo, hi);
+              pk[e] = pack_bf16(pr[e]);
+              if (kCap) pr[e] = mul2(pr[e], slope);
             }
           }
         };
-        auto gradients = [&](auto m, int c) {
+        auto gradients = [&](auto m) {
 #pragma unroll
-          for (int i4 = 0; i4 < 8; ++i4) {
-            const float4 l = stat[32 + c * 8 + i4];
-            const float dl[4] = {l.x, l.y, l.z, l.w};
-            float last = 0.0f;
+          for (int i = 0; i < 32; i += 2) {
+            const float4 l = stat[32 + (i >> 1)];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int q = c * 32 + i4 * 4 + e;
-              float d = pr[q] * (__uint_as_float(v[i4 * 4 + e]) - dl[e]);
-              if (decltype(m)::value && (q < lo || q >= hi)) d = 0.0f;
-              if (e & 1) pk[q >> 1] = pack_bf16(last, d);
-              last = d;
+            for (int e = i; e < i + 2; ++e) {
+              const Pair dp = e < 16 ? make_pair(v[(2 * e) & 31], v[(2 * e + 1) & 31]) : make_pair(u[(2 * e) & 31], u[(2 * e + 1) & 31]);
+              Pair d = mul2(pr[e], add2(dp, e == i ? make_pair(l.x, l.y) : make_pair(l.z, l.w)));
+              if (decltype(m)::value) d = keep_range(d, 2 * e, lo, hi);
+              pk[e] = pack_bf16(d);
             }
           }
         };
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          tc_ld_32x32b_x32(s_addr + c * 32, v);
-          tc_wait_ld();
-          // one branch per tile: the tests of a masked tile cost as much as the arithmetic
-          if (masked) probabilities(TrueTag{}, c);
-          else probabilities(FalseTag{}, c);
-        }
+        tc_ld_32x32b_x32(s_addr, v);
+        tc_ld_32x32b_x32(s_addr + 32, u);
+        tc_wait_ld();
+        if (masked) probabilities(TrueTag{});
+        else probabilities(FalseTag{});
         tc_st_32x32b_x32(s_addr, pk);
         tc_wait_st();
         tc_fence_before();
-        mbar_arrive(BAR(p_full));
+        warp_arrive(BAR(p_full));
         if (!warp_wait(BAR(dp_full), n & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 452)) { ok = false; break; }
         tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          tc_ld_32x32b_x32(dp_addr + c * 32, v);
-          tc_wait_ld();
-          if (masked) gradients(TrueTag{}, c);
-          else gradients(FalseTag{}, c);
-        }
+        tc_ld_32x32b_x32(dp_addr, v);
+        tc_ld_32x32b_x32(dp_addr + 32, u);
+        tc_wait_ld();
+        if (masked) gradients(TrueTag{});
+        else gradients(FalseTag{});
         tc_st_32x32b_x32(dp_addr, pk);
         tc_wait_st();
         tc_fence_before();
-        mbar_arrive(BAR(ds_full));
-        __syncwarp();
-        if (lane == 0) mbar_arrive(BAR(stat_empty) + 8 * ss);
+        warp_arrive(BAR(ds_full));
+        warp_arrive(BAR(stat_empty) + 8 * ss);
       }
       if (!ok) break;
       if (!warp_wait(BAR(acc_full), it & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 453)) { ok = false; break; }
       tc_fence_after();
-      const size_t at = ((static_cast<size_t>(t.b) * p.seq + k_pos) * p.kv_heads + t.h) * kD + half * 64;
       uint32_t a[32], b[32];
       tc_ld_32x32b_x32(t_dv + lane_addr + half * 64, a);
       tc_ld_32x32b_x32(t_dv + lane_addr + half * 64 + 32, b);
       tc_wait_ld();
-      if (k_pos < p.seq) store_half_row(a, b, 1.0f, p.dv + at);
-      tc_ld_32x32b_x32(t_dk + lane_addr + half * 64, a);
-      tc_ld_32x32b_x32(t_dk + lane_addr + half * 64 + 32, b);
-      tc_wait_ld();
-      tc_fence_before();
-      mbar_arrive(BAR(acc_free));
+      if (walk.i0 == 0 && walk.i1 == t.n) {
+        const size_t at = ((static_cast<size_t>(t.b) * p.seq + k_pos) * p.kv_heads + t.h) * kD + half * 64;
+        if (k_pos < p.seq) store_half_row(a, b, 1.0f, p.dv + at);
+        tc_ld_32x32b_x32(t_dk + lane_addr + half * 64, a);
+        tc_ld_32x32b_x32(t_dk + lane_addr + half * 64 + 32, b);
+        tc_wait_ld();
+        tc_fence_before();
+        warp_arrive(BAR(acc_free));
+        if (k_pos < p.seq) store_half_row(a, b, p.scale, p.dk + at);
+      } else {
+        // part of a tile: fp32 sums for the joining kernel, 4 columns of all rows together
+        float4* part = p.partial + (2 * static_cast<size_t>(blockIdx.x) + (walk.i0 == 0 ? 1 : 0)) * kPartVecs + half * 16 * kBlk + row;
+        store_part(a, b, part);
+        tc_ld_32x32b_x32(t_dk + lane_addr + half * 64, a);
+        tc_ld_32x32b_x32(t_dk + lane_addr + half * 64 + 32, b);
+        tc_wait_ld();
+        tc_fence_before();
+        warp_arrive(BAR(acc_free));
+        store_part(a, b, part + kPartVecs / 2);
+      }
       ++it;
-      if (k_pos < p.seq) store_half_row(a, b, p.scale, p.dk + at);
     }
   }
 #undef BAR
@@ -662,6 +793,69 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// Tiles that more than one run worked on: block (c, y) takes the tile whose first cut is where run c begins, and an
+// eighth of its columns; the parts are added in the order of their runs.
+__global__ void __launch_bounds__(256)
+attention_bwd_join_kernel(const AttnBwdParams p) {
+  const int c = blockIdx.x + 1;
+  int w, step;
+  const int64_t at = run_begin(p, c);
+  locate(p, at, w, step);
+  const int64_t begin = at - step;
+  if (step == 0 || run_begin(p, c - 1) > begin) return;      // no cut, or not the tile's first
+  const KvItem t = kv_item(p, w);
+  int last = c;                                              // the last run with steps of this tile
+  while (last + 1 < p.parts && run_begin(p, last + 1) < begin + t.n) ++last;
+  const int row = threadIdx.x & (kBlk - 1);
+  if (t.k0 + row >= p.seq) return;
+  // 64 column groups of 4 (dV, dK) over 8 blocks and two halves of the CTA: 4 a thread, stored in pairs
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int group = blockIdx.y * 8 + (threadIdx.x >> 7) * 4 + k * 2;
+    float s[8];
+    const float4* part = p.partial + (2 * static_cast<size_t>(c - 1) + 1) * kPartVecs + group * kBlk + row;
+    float4 u = part[0], v = part[kBlk];
+    s[0] = u.x; s[1] = u.y; s[2] = u.z; s[3] = u.w; s[4] = v.x; s[5] = v.y; s[6] = v.z; s[7] = v.w;
+    for (int r = c; r <= last; ++r) {
+      part = p.partial + 2 * static_cast<size_t>(r) * kPartVecs + group * kBlk + row;
+      u = part[0];
+      v = part[kBlk];
+      s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w; s[4] += v.x; s[5] += v.y; s[6] += v.z; s[7] += v.w;
+    }
+    const bool dk = group >= 32;
+    const float scale = dk ? p.scale : 1.0f;
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const __nv_bfloat162 x = __floats2bfloat162_rn(s[2 * e] * scale, s[2 * e + 1] * scale);
+      o[e] = *reinterpret_cast<const uint32_t*>(&x);
+    }
+    __nv_bfloat16* dst = (dk ? p.dk : p.dv) + ((static_cast<size_t>(t.b) * p.seq + t.k0 + row) * p.kv_heads + t.h) * kD + (group & 31) * 4;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// How the second kernel shares its work out. Whole tiles to CTAs leave SMs idle when there are few tiles (causal
+// tiles differ in length by their number) or the last wave is short; equal runs of steps leave none idle and cost
+// the parts' fp32 sums and the joining kernel, about ten steps' time. Measured at 2048 positions, 32 / 8 heads:
+// kPlanNote.
+struct KvPlan { int parts; int64_t steps; };
+KvPlan kv_plan(int batch, int seq, int kv_heads, int group, int window) {
+  const int tiles = (seq + kBlk - 1) / kBlk;
+  const int64_t bh = static_cast<int64_t>(batch) * kv_heads;
+  KvPlan plan = {0, 0};
+  for (int kb = 0; kb < tiles; ++kb) plan.steps += kv_query_tiles(tiles, window, kb);
+  plan.steps *= bh * group;
+  const int64_t items = tiles * bh, longest = static_cast<int64_t>(kv_query_tiles(tiles, window, 0)) * group;
+  const int64_t even = plan.steps / kBwdRuns, waves = (items + kBwdRuns - 1) / kBwdRuns;
+  int64_t whole = even + longest / 8;
+  if (whole < longest) whole = longest;
+  if (whole < waves * plan.steps / items) whole = waves * plan.steps / items;
+  if (whole > even + 10) plan.parts = static_cast<int>(plan.steps / 8 < kBwdRuns ? plan.steps / 8 : kBwdRuns);
+  if (plan.parts < 2) plan.parts = 0;
+  return plan;
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -690,6 +884,12 @@ bool encode_sequences(CUtensorMap* map, const void* base, uint64_t batch, uint64
 
 }  // namespace
 
+size_t attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv_heads, int window) {
+  const size_t rows = static_cast<size_t>(batch) * q_heads * ((static_cast<size_t>(seq) + kBlk - 1) / kBlk * kBlk);
+  const KvPlan plan = kv_plan(batch, seq, kv_heads, q_heads / kv_heads, window < seq ? window : 0);
+  return kBwdStatusBytes + 2 * rows * sizeof(float) + static_cast<size_t>(plan.parts) * 2 * kPartVecs * sizeof(float4);
+}
+
 cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream) {
   CUtensorMap mq, mdo, mk, mv;
   if (!encode_sequences(&mq, a.q, a.batch, a.seq, static_cast<uint64_t>(a.q_heads) * kD) ||
@@ -712,14 +912,24 @@ cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream) {
   p.kv_heads = a.kv_heads;
   p.group = a.q_heads / a.kv_heads;
   p.window = a.window < a.seq ? a.window : 0;     // a window no shorter than the sequence hides nothing
-  p.lse2 = a.workspace;
-  p.delta = a.workspace + static_cast<int64_t>(a.batch) * a.q_heads * p.seq_pad;
+  // the workspace: a status record for callers without one, the row constants, the parts of cut tiles
+  p.lse2 = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kBwdStatusBytes);
+  p.delta = p.lse2 + static_cast<int64_t>(a.batch) * a.q_heads * p.seq_pad;
+  p.partial = reinterpret_cast<float4*>(p.delta + static_cast<int64_t>(a.batch) * a.q_heads * p.seq_pad);
+  const KvPlan plan = kv_plan(a.batch, a.seq, a.kv_heads, p.group, p.window);
+  p.parts = plan.parts;
+  p.steps = plan.steps;
   p.scale = a.scale;
   p.scale_log2 = a.scale * kLog2e;
   const bool cap = a.softcap > 0.0f;
   p.cap_in = cap ? 2.0f * kLog2e * a.scale / a.softcap : 0.0f;
   p.cap_out = a.softcap * kLog2e;
   p.status = a.status;
+  if (p.status == nullptr) {
+    p.status = static_cast<Status*>(a.workspace);
+    const cudaError_t zeroed = cudaMemsetAsync(a.workspace, 0, sizeof(Status), stream);
+    if (zeroed != cudaSuccess) return zeroed;
+  }
   const int64_t q_items = static_cast<int64_t>(p.tiles) * a.batch * a.q_heads;
   const int64_t kv_items = static_cast<int64_t>(p.tiles) * a.batch * a.kv_heads;
   auto dq = cap ? attention_bwd_dq_kernel<true> : attention_bwd_dq_kernel<false>;
@@ -731,7 +941,11 @@ cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream) {
   dq<<<static_cast<int>(q_items < a.num_sms ? q_items : a.num_sms), kBwdThreads, kDqSmem, stream>>>(mq, mdo, mk, mv, p);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
-  dkdv<<<static_cast<int>(kv_items < a.num_sms ? kv_items : a.num_sms), kBwdThreads, kKvSmem, stream>>>(mq, mdo, mk, mv, p);
+  const int grid = p.parts > 0 ? p.parts : static_cast<int>(kv_items < a.num_sms ? kv_items : a.num_sms);
+  dkdv<<<grid, kBwdThreads, kKvSmem, stream>>>(mq, mdo, mk, mv, p);
+  err = cudaGetLastError();
+  if (err != cudaSuccess || p.parts == 0) return err;
+  attention_bwd_join_kernel<<<dim3(p.parts - 1, 8), 256, 0, stream>>>(p);
   return cudaGetLastError();
 }
 

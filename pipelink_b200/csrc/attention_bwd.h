@@ -11,8 +11,8 @@ struct AttnBwdParams {
   const __nv_bfloat16* out;
   const __nv_bfloat16* d_out;
   const float* lse;          // [batch * q_heads, seq], natural log
-  float* lse2;               // [batch * q_heads, seq_pad]: base 2, +inf where a row has no probabilities
-  float* delta;              // [batch * q_heads, seq_pad]
+  float* lse2;               // [batch * q_heads, seq_pad]: base 2 and negated, -inf where a row has no probabilities
+  float* delta;              // [batch * q_heads, seq_pad], negated
   __nv_bfloat16* dq;
   __nv_bfloat16* dk;
   __nv_bfloat16* dv;
@@ -21,21 +21,28 @@ struct AttnBwdParams {
   int window;                // 0 = none
   float scale, scale_log2;
   float cap_in, cap_out;     // soft cap: y = cap_out * tanh in base 2, 2 log2(e) * scale / cap on the way in
+  // dK, dV: runs of steps (0: whole tiles to CTAs) and the steps in all; two slots of fp32 sums a run
+  int parts;
+  int64_t steps;
+  float4* partial;
   Status* status;
 };
+
+constexpr int kBwdStatusBytes = 256;
 
 struct AttnBwdArgs {
   const void *q, *k, *v, *out, *d_out;
   const float* lse;
   void *dq, *dk, *dv;
-  float* workspace;          // 2 * batch * q_heads * (seq rounded up to 128) floats, 16-byte aligned
+  void* workspace;           // attention_bwd_workspace_bytes(), 16-byte aligned
   int batch, seq, q_heads, kv_heads;
   float scale, softcap;
   int window;
   int num_sms;
-  Status* status;
+  Status* status;            // null: one in the workspace, which nobody reads
 };
 
+size_t attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv_heads, int window);
 cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream);
 
 }  // namespace plb

@@ -1015,28 +1015,31 @@ int plb_tensor_map_2d_u32(void* out128, const void* base, uint64_t rows, uint64_
   return PLB_OK;
 }
 
-size_t plb_attention_bwd_workspace_bytes(int batch, int seq, int q_heads) {
-  if (batch < 0 || seq < 0 || q_heads < 0) return 0;
-  return static_cast<size_t>(2) * batch * q_heads * ((static_cast<size_t>(seq) + 127) / 128 * 128) * sizeof(float);
+static bool attention_bwd_shape_ok(int batch, int seq, int q_heads, int kv_heads, int window) {
+  if (batch < 0 || seq < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || window < 0) return false;
+  // tiles and work items are counted in 32 bits
+  return seq <= (1 << 30) && (static_cast<int64_t>(seq) + 127) / 128 * batch * q_heads <= (1 << 30);
+}
+
+size_t plb_attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv_heads, int window) {
+  if (!attention_bwd_shape_ok(batch, seq, q_heads, kv_heads, window) || batch == 0 || seq == 0) return 0;
+  return plb::attention_bwd_workspace_bytes(batch, seq, q_heads, kv_heads, window);
 }
 
 int plb_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* d_out, const float* lse,
                       void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, int batch, int seq, int q_heads,
                       int kv_heads, float scale, int window, float softcap, plb_status* status, void* stream) {
-  if (batch < 0 || seq < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || window < 0 || !(softcap >= 0.0f))
-    return PLB_E_ARGUMENT;
+  if (!attention_bwd_shape_ok(batch, seq, q_heads, kv_heads, window) || !(softcap >= 0.0f)) return PLB_E_ARGUMENT;
   if (batch == 0 || seq == 0) return PLB_OK;
-  if (!q || !k || !v || !out || !d_out || !lse || !dq || !dk || !dv || !workspace || !status) return PLB_E_ARGUMENT;
+  if (!q || !k || !v || !out || !d_out || !lse || !dq || !dk || !dv || !workspace) return PLB_E_ARGUMENT;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(d_out) || !aligned16(dq) ||
       !aligned16(dk) || !aligned16(dv) || !aligned16(workspace))
     return PLB_E_ARGUMENT;
-  if (workspace_bytes < plb_attention_bwd_workspace_bytes(batch, seq, q_heads)) return PLB_E_CAPACITY;
-  // tiles and work items are counted in 32 bits
-  if (seq > (1 << 30) || (static_cast<int64_t>(seq) + 127) / 128 * batch * q_heads > (1 << 30)) return PLB_E_ARGUMENT;
+  if (workspace_bytes < plb::attention_bwd_workspace_bytes(batch, seq, q_heads, kv_heads, window)) return PLB_E_CAPACITY;
   plb::AttnBwdArgs a;
   a.q = q; a.k = k; a.v = v; a.out = out; a.d_out = d_out; a.lse = lse;
   a.dq = dq; a.dk = dk; a.dv = dv;
-  a.workspace = static_cast<float*>(workspace);
+  a.workspace = workspace;
   a.batch = batch; a.seq = seq; a.q_heads = q_heads; a.kv_heads = kv_heads;
   a.scale = scale; a.window = window; a.softcap = softcap;
   a.num_sms = sm_count();

@@ -9,12 +9,14 @@ OK, CAPACITY, ARGUMENT = 0, 2, 3
 
 
 def bwd(lib, *, batch=1, seq=256, q_heads=4, kv_heads=2, window=0, softcap=0.0, nbytes=None, ptr=4096, last=4096):
-    n = lib.plb_attention_bwd_workspace_bytes(batch, seq, q_heads) if nbytes is None else nbytes
+    n = lib.plb_attention_bwd_workspace_bytes(batch, seq, q_heads, kv_heads, max(window, 0)) if nbytes is None else nbytes
     return lib.plb_attention_bwd(*[P(ptr)] * 9, P(last), n, batch, seq, q_heads, kv_heads, 1.0, window, softcap, P(ptr), None)
 
 
 def test_attention_bwd_refusals(native_lib):
-    assert native_lib.plb_attention_bwd_workspace_bytes(2, 129, 3) == 2 * 2 * 3 * 256 * 4
+    need = native_lib.plb_attention_bwd_workspace_bytes
+    assert need(2, 129, 3, 1, 0) >= 2 * 2 * 3 * 256 * 4 and need(1, 8192, 32, 8, 0) >= 2 * 32 * 8192 * 4
+    assert need(0, 129, 3, 1, 0) == 0 and need(2, 129, 3, 2, 0) == 0 and need(1, 128, 1, 1, -1) == 0
     for bad in (dict(batch=-1), dict(seq=-1), dict(q_heads=0), dict(kv_heads=0), dict(q_heads=5), dict(window=-1), dict(softcap=-1.0),
                 dict(softcap=float("nan")), dict(ptr=None), dict(ptr=4104), dict(last=None), dict(seq=2 ** 30 + 1), dict(batch=2 ** 23, seq=2 ** 20)):
         assert bwd(native_lib, **bad) in (ARGUMENT, CAPACITY), bad
