@@ -44,10 +44,13 @@ constexpr int kDqRed = kDqV + kDqVStages * kTileBytes;                // [2][2][
 constexpr int kDqBar = kDqRed + 2048;
 constexpr int kDqSmem = kDqBar + 256;
 
-constexpr int kKvQ = 2 * kTileBytes, kKvQStages = 3;                  // after K and V
-constexpr int kKvDo = kKvQ + kKvQStages * kTileBytes, kKvDoStages = 2;
-constexpr int kKvStat = kKvDo + kKvDoStages * kTileBytes, kKvStatStages = 2;   // 128 lse2, 128 delta
-constexpr int kKvBar = kKvStat + kKvStatStages * 1024;
+// dK, dV: K and V, then the streamed tiles with their rows' constants behind them (see kAuxBytes)
+constexpr int kAuxBytes = kBlk * 32;                                  // 128 rows of 16 bf16
+constexpr int kKvStage = kTileBytes + kAuxBytes;
+constexpr int kKvQ = 2 * kTileBytes, kKvQStages = 2;
+constexpr int kKvDo = kKvQ + kKvQStages * kKvStage, kKvDoStages = 2;
+constexpr int kKvOnes = kKvDo + kKvDoStages * kKvStage;
+constexpr int kKvBar = kKvOnes + kAuxBytes;
 constexpr int kKvSmem = kKvBar + 256;
 static_assert(kDqSmem <= 232448 && kKvSmem <= 232448, "227 KB of shared memory per CTA");
 
@@ -58,7 +61,6 @@ struct DqBars {
 };
 struct KvBars {
   uint64_t kv_full, kv_empty, q_full[kKvQStages], q_empty[kKvQStages], do_full[kKvDoStages], do_empty[kKvDoStages];
-  uint64_t stat_full[kKvStatStages], stat_empty[kKvStatStages];
   uint64_t s_full, p_full, dp_full, ds_full, acc_full, acc_free, drain;
   uint32_t tmem_base, pad;
 };
@@ -100,58 +102,57 @@ __device__ __forceinline__ KvItem kv_item(const AttnBwdParams& p, int w) {
   t.n = t.tiles * p.group;
   return t;
 }
-// The key tiles' steps (a step: one query tile of one head) in one line, heaviest tiles first, cut into p.parts equal
-// runs: where run r begins, as a tile and a step of it.
-__device__ __forceinline__ int64_t run_begin(const AttnBwdParams& p, int r) { return p.steps * r / p.parts; }
-__device__ __forceinline__ void locate(const AttnBwdParams& p, int64_t at, int& w, int& step) {
+// The key tiles' steps (a step: one query tile of one head) in one line, heaviest tiles first, cut into p.parts runs
+// of equal time, where a tile counts kTileSteps more than it has, for its loads and stores: where run r begins, as a
+// tile and a step of it.
+constexpr int kTileSteps = 2;
+__device__ __forceinline__ void run_begin(const AttnBwdParams& p, int r, int& w, int& step) {
   const int bh = p.batch * p.kv_heads;
-  for (int kb = 0;; ++kb) {
-    const int n = kv_query_tiles(p.tiles, p.window, kb) * p.group;
-    if (at < static_cast<int64_t>(n) * bh || kb == p.tiles - 1) {
-      const int r = static_cast<int>(at / n);
-      w = kb * bh + r;
-      step = static_cast<int>(at - static_cast<int64_t>(r) * n);
+  int64_t at = p.steps * r / p.parts;
+  for (int kb = 0; kb < p.tiles; ++kb) {
+    const int n = kv_query_tiles(p.tiles, p.window, kb) * p.group + kTileSteps;
+    if (at < static_cast<int64_t>(n) * bh) {
+      const int i = static_cast<int>(at / n);
+      w = kb * bh + i;
+      step = max(0, static_cast<int>(at - static_cast<int64_t>(i) * n) - kTileSteps);
       return;
     }
     at -= static_cast<int64_t>(n) * bh;
   }
+  w = p.tiles * bh;
+  step = 0;
 }
 // What a CTA works through: whole tiles (parts 0, the list walked forth and back) or its run, steps [i0, i1) of tile w.
 struct KvWalk {
-  int w, i0, i1, wave;
-  int64_t left;
+  int w, i0, i1, wave, end_w, end_step;
   KvItem t;
   __device__ __forceinline__ bool begin(const AttnBwdParams& p, int items) {
     wave = 0;
-    left = 0;
     i0 = 0;
+    end_w = items;
+    end_step = 0;
     if (p.parts > 0) {
-      left = run_begin(p, blockIdx.x + 1) - run_begin(p, blockIdx.x);
-      locate(p, run_begin(p, blockIdx.x), w, i0);
-      if (left <= 0) return false;
+      run_begin(p, blockIdx.x, w, i0);
+      run_begin(p, blockIdx.x + 1, end_w, end_step);
     } else {
       w = snake(0);
-      if (w >= items) return false;
     }
-    set(p);
-    return true;
+    return set(p);
   }
-  __device__ __forceinline__ bool next(const AttnBwdParams& p, int items) {
+  __device__ __forceinline__ bool next(const AttnBwdParams& p) {
     if (p.parts > 0) {
-      left -= i1 - i0;
-      if (left <= 0) return false;
       ++w;
       i0 = 0;
     } else {
       w = snake(++wave);
-      if (w >= items) return false;      // only the last wave is short
     }
-    set(p);
-    return true;
+    return set(p);
   }
-  __device__ __forceinline__ void set(const AttnBwdParams& p) {
+  __device__ __forceinline__ bool set(const AttnBwdParams& p) {
+    if (w > end_w || (w == end_w && i0 >= end_step)) return false;     // only the last wave of whole tiles is short
     t = kv_item(p, w);
-    i1 = p.parts > 0 && left < t.n - i0 ? i0 + static_cast<int>(left) : t.n;
+    i1 = w == end_w ? end_step : t.n;
+    return true;
   }
 };
 
@@ -169,15 +170,34 @@ __device__ __forceinline__ void warp_commit(uint32_t bar) {
   if (elect_one_sync()) tc_commit(bar);
   __syncwarp();
 }
-// D = A B^T over 128 columns of the contraction, both operands K-major tiles in shared memory, then the barrier.
-__device__ __forceinline__ void mma_tiles(uint32_t d, uint32_t a, uint32_t b, uint32_t bar) {
+// A constant c_q of every row q of B, added to column q of A B^T by the tensor core: one more step of the contraction
+// whose A is all ones and whose B row holds c_q as three bf16 numbers (24 bits, an fp32 number) and zeros. In the
+// transposed products the constants belong to columns, and every thread would read all 128 of them from shared
+// memory, 665 cycles of its bandwidth a tile next to the 2048 the products take.
+constexpr uint64_t kDescAux = smem_desc_hi(256, 0, 6);                // rows of 32 bytes, 32-byte swizzle
+__device__ __forceinline__ void store_constant(uint8_t* tile, int row, float c) {
+  const __nv_bfloat16 hi = __float2bfloat16_rn(c);
+  const float r = fabsf(c) < INFINITY ? c - __bfloat162float(hi) : 0.0f;
+  const __nv_bfloat16 mid = __float2bfloat16_rn(r);
+  const __nv_bfloat16 lo = __float2bfloat16_rn(r - __bfloat162float(mid));
+  const uint32_t w0 = static_cast<uint32_t>(__bfloat16_as_ushort(hi)) | static_cast<uint32_t>(__bfloat16_as_ushort(mid)) << 16;
+  uint4* dst = reinterpret_cast<uint4*>(tile + row * 32);
+  const int first = (row >> 2) & 1;                                   // the swizzle exchanges the two 16-byte chunks of rows 4-7 of 8
+  dst[first] = make_uint4(w0, __bfloat16_as_ushort(lo), 0, 0);
+  dst[first ^ 1] = make_uint4(0, 0, 0, 0);
+}
+// D = A B^T over 128 columns of the contraction, both operands K-major tiles in shared memory, then the barrier. With
+// aux, B's rows' constants are added (ones: the tile of ones).
+__device__ __forceinline__ void mma_tiles(uint32_t d, uint32_t a, uint32_t b, uint32_t bar, uint32_t ones = 0, uint32_t aux = 0) {
   const uint64_t ad = smem_desc(a, kDescSw128KMajor), bd = smem_desc(b, kDescSw128KMajor);
+  const uint64_t od = smem_desc(ones, kDescAux), cd = smem_desc(aux, kDescAux);
   if (elect_one_sync()) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const uint32_t off = ((k >> 2) * kAtomBytes + (k & 3) * 32) >> 4;
       tc_mma_f16(d, ad + off, bd + off, kIdescQK, k != 0 ? 1u : 0u);
     }
+    if (aux != 0) tc_mma_f16(d, od, cd, kIdescQK, 1u);
     tc_commit(bar);
   }
   __syncwarp();
@@ -273,19 +293,41 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&t);
 }
-// 64 fp32 accumulator columns of this lane, scaled, as bf16 to 128 contiguous bytes.
-__device__ __forceinline__ void store_half_row(const uint32_t (&a)[32], const uint32_t (&b)[32], float scale, __nv_bfloat16* dst) {
-  uint4* out = reinterpret_cast<uint4*>(dst);
+// 64 fp32 accumulator columns of each lane's row, scaled, as bf16 to 128 bytes of the row; `rows` of the warp's rows
+// exist, `stride` elements apart from dst on. Eight lanes first exchange their 16-byte chunks so that each store
+// writes whole 128-byte pieces of four rows; a lane storing its own row would touch 32 lines with every store, some
+// 8000 cycles of the store path a tile.
+__device__ __forceinline__ void store_half_rows(const uint32_t (&a)[32], const uint32_t (&b)[32], float scale, __nv_bfloat16* dst,
+                                                int64_t stride, int rows) {
+  const int lane = threadIdx.x & 31;
+  uint32_t w[8][4];
 #pragma unroll
-  for (int g = 0; g < 8; ++g) {
-    uint32_t w[4];
+  for (int g = 0; g < 8; ++g)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = (g & 3) * 8 + e * 2;
-      w[e] = g < 4 ? pack_bf16(__uint_as_float(a[i]) * scale, __uint_as_float(a[i + 1]) * scale)
-                   : pack_bf16(__uint_as_float(b[i]) * scale, __uint_as_float(b[i + 1]) * scale);
+      w[g][e] = g < 4 ? pack_bf16(mul2(make_pair(a[i], a[i + 1]), make_pair(scale, scale)))
+                      : pack_bf16(mul2(make_pair(b[i], b[i + 1]), make_pair(scale, scale)));
     }
-    out[g] = make_uint4(w[0], w[1], w[2], w[3]);
+  // chunk g of lane l goes to chunk l of lane g of its eight: exchange across one bit of both at a time
+#pragma unroll
+  for (int bit = 1; bit < 8; bit <<= 1) {
+    const bool up = lane & bit;
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      if (g & bit) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t got = __shfl_xor_sync(kFullMask, up ? w[g][e] : w[g | bit][e], bit);
+        if (up) w[g][e] = got;
+        else w[g | bit][e] = got;
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {
+    const int row = (lane & ~7) + g;
+    if (row < rows) reinterpret_cast<uint4*>(dst + row * stride)[lane & 7] = make_uint4(w[g][0], w[g][1], w[g][2], w[g][3]);
   }
 }
 
@@ -475,10 +517,12 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       warp_arrive(BAR(red));
       if (!warp_wait(BAR(red), it & 1u, p.status, ST_TIMEOUT_FULL, 423)) { ok = false; break; }
       const float delta = red_it[row] + red_it[kBlk + row];
-      if (half == 0) {
-        const int64_t at = (static_cast<int64_t>(t.b) * p.q_heads + t.h) * p.seq_pad + q_pos;
-        p.lse2[at] = -r.lse2;
-        p.delta[at] = -delta;
+      {
+        // for the second kernel: -delta, and the log-sum-exp as it enters S (with a cap: as it is subtracted from y)
+        const int64_t tile = ((static_cast<int64_t>(t.b) * p.q_heads + t.h) * p.seq_pad + t.q0) * 32;
+        if (half != 0) store_constant(p.delta + tile, row, -delta);
+        else if (kCap) *reinterpret_cast<float*>(p.lse2 + tile / 8 + row * 4) = -r.lse2;
+        else store_constant(p.lse2 + tile, row, -r.lse2 * p.inv_scale_log2);
       }
       const Pair minus_lse2 = make_pair(-r.lse2, -r.lse2), minus_delta = make_pair(-delta, -delta);
       for (int j = 0; j < t.blocks; ++j, ++blk) {
@@ -536,7 +580,9 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       tc_fence_before();
       warp_arrive(BAR(dq_free));
       ++it;
-      if (r.live) store_half_row(a, b, p.scale, p.dq + r.at);
+      const int row0 = t.q0 + quad * 32;
+      store_half_rows(a, b, p.scale, p.dq + ((static_cast<size_t>(t.b) * p.seq + row0) * p.q_heads + t.h) * kD + half * 64,
+                      static_cast<int64_t>(p.q_heads) * kD, p.seq - row0);
     }
   }
 #undef BAR
@@ -571,7 +617,6 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     mbar_init(BAR(kv_empty), 1);
     for (int s = 0; s < kKvQStages; ++s) { mbar_init(BAR(q_full) + 8 * s, 1); mbar_init(BAR(q_empty) + 8 * s, 1); }
     for (int s = 0; s < kKvDoStages; ++s) { mbar_init(BAR(do_full) + 8 * s, 1); mbar_init(BAR(do_empty) + 8 * s, 1); }
-    for (int s = 0; s < kKvStatStages; ++s) { mbar_init(BAR(stat_full) + 8 * s, 1); mbar_init(BAR(stat_empty) + 8 * s, kComputeWarps); }
     mbar_init(BAR(s_full), 1);
     mbar_init(BAR(p_full), kComputeWarps);
     mbar_init(BAR(dp_full), 1);
@@ -585,6 +630,8 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
   }
+  for (int i = threadIdx.x; i < kAuxBytes / 4; i += kBwdThreads) reinterpret_cast<uint32_t*>(smem + kKvOnes)[i] = 0x3F803F80u;
+  fence_proxy_async_smem();
   if (warp == 1) {
     tmem_alloc(smem_u32(&bars->tmem_base), 512);
     tmem_relinquish();
@@ -600,7 +647,7 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     uint32_t it = 0, n = 0;
     bool ok = true;
     KvWalk walk;
-    for (bool go = walk.begin(p, items); go && ok; go = walk.next(p, items)) {
+    for (bool go = walk.begin(p, items); go && ok; go = walk.next(p)) {
       const KvItem& t = walk.t;
       if (!warp_wait(BAR(kv_empty), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_EMPTY, 430)) { ok = false; break; }
       if (elect_one_sync()) {
@@ -613,25 +660,22 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       int g = walk.i0 / t.tiles, qt = walk.i0 % t.tiles;
       for (int i = walk.i0; i < walk.i1; ++i, ++n) {
         const int h = t.h * p.group + g, row = (t.first + qt) * kBlk;
-        const uint32_t qs = n % kKvQStages, ds = n % kKvDoStages, ss = n % kKvStatStages;
+        const uint32_t qs = n % kKvQStages, ds = n % kKvDoStages;
+        const uint32_t q_dst = sb + kKvQ + qs * kKvStage, do_dst = sb + kKvDo + ds * kKvStage;
+        const int64_t at = ((static_cast<int64_t>(t.b) * p.q_heads + h) * p.seq_pad + row) * 32;
         if (!warp_wait(BAR(q_empty) + 8 * qs, ((n / kKvQStages) & 1u) ^ 1u, p.status, ST_TIMEOUT_EMPTY, 431)) { ok = false; break; }
         if (elect_one_sync()) {
-          mbar_arrive_expect_tx(BAR(q_full) + 8 * qs, kTileBytes);
-          load_tile(sb + kKvQ + qs * kTileBytes, &map_q, BAR(q_full) + 8 * qs, h * kD, row, t.b);
-        }
-        __syncwarp();
-        if (!warp_wait(BAR(stat_empty) + 8 * ss, ((n / kKvStatStages) & 1u) ^ 1u, p.status, ST_TIMEOUT_EMPTY, 432)) { ok = false; break; }
-        if (elect_one_sync()) {
-          const int64_t at = (static_cast<int64_t>(t.b) * p.q_heads + h) * p.seq_pad + row;
-          mbar_arrive_expect_tx(BAR(stat_full) + 8 * ss, 1024);
-          bulk_load(sb + kKvStat + ss * 1024, p.lse2 + at, 512, BAR(stat_full) + 8 * ss);
-          bulk_load(sb + kKvStat + ss * 1024 + 512, p.delta + at, 512, BAR(stat_full) + 8 * ss);
+          constexpr int kLseBytes = kCap ? kBlk * 4 : kAuxBytes;
+          mbar_arrive_expect_tx(BAR(q_full) + 8 * qs, kTileBytes + kLseBytes);
+          load_tile(q_dst, &map_q, BAR(q_full) + 8 * qs, h * kD, row, t.b);
+          bulk_load(q_dst + kTileBytes, p.lse2 + (kCap ? at / 8 : at), kLseBytes, BAR(q_full) + 8 * qs);
         }
         __syncwarp();
         if (!warp_wait(BAR(do_empty) + 8 * ds, ((n / kKvDoStages) & 1u) ^ 1u, p.status, ST_TIMEOUT_EMPTY, 433)) { ok = false; break; }
         if (elect_one_sync()) {
-          mbar_arrive_expect_tx(BAR(do_full) + 8 * ds, kTileBytes);
-          load_tile(sb + kKvDo + ds * kTileBytes, &map_do, BAR(do_full) + 8 * ds, h * kD, row, t.b);
+          mbar_arrive_expect_tx(BAR(do_full) + 8 * ds, kTileBytes + kAuxBytes);
+          load_tile(do_dst, &map_do, BAR(do_full) + 8 * ds, h * kD, row, t.b);
+          bulk_load(do_dst + kTileBytes, p.delta + at, kAuxBytes, BAR(do_full) + 8 * ds);
         }
         __syncwarp();
         if (++qt == t.tiles) { qt = 0; ++g; }
@@ -645,37 +689,40 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       const uint32_t qs = i % kKvQStages;
       if (!warp_wait(BAR(q_full) + 8 * qs, (i / kKvQStages) & 1u, p.status, ST_TIMEOUT_FULL, 440)) return false;
       tc_fence_after();
-      mma_tiles(t_s, sb, sb + kKvQ + qs * kTileBytes, BAR(s_full));
+      const uint32_t q = sb + kKvQ + qs * kKvStage;
+      mma_tiles(t_s, sb, q, BAR(s_full), sb + kKvOnes, kCap ? 0 : q + kTileBytes);
       return true;
     };
     auto issue_dp = [&](uint32_t i) {
       const uint32_t ds = i % kKvDoStages;
       if (!warp_wait(BAR(do_full) + 8 * ds, (i / kKvDoStages) & 1u, p.status, ST_TIMEOUT_FULL, 441)) return false;
       tc_fence_after();
-      mma_tiles(t_dp, sb + kTileBytes, sb + kKvDo + ds * kTileBytes, BAR(dp_full));
+      const uint32_t g = sb + kKvDo + ds * kKvStage;
+      mma_tiles(t_dp, sb + kTileBytes, g, BAR(dp_full), sb + kKvOnes, g + kTileBytes);
       return true;
     };
     KvWalk walk;
-    for (bool go = walk.begin(p, items); go && ok; go = walk.next(p, items)) {
+    for (bool go = walk.begin(p, items); go && ok; go = walk.next(p)) {
       const int steps = __shfl_sync(kFullMask, walk.i1 - walk.i0, 0);
       if (!warp_wait(BAR(kv_full), it & 1u, p.status, ST_TIMEOUT_FULL, 442)) { ok = false; break; }
       tc_fence_after();
       if (!issue_s(n) || !issue_dp(n)) { ok = false; break; }
+      if (steps == 1) warp_commit(BAR(kv_empty));
       for (int i = 0; i < steps && ok; ++i, ++n) {
         const bool more = i + 1 < steps;
         const uint32_t qs = n % kKvQStages, ds = n % kKvDoStages;
         if (!warp_wait(BAR(p_full), n & 1u, p.status, ST_TIMEOUT_FULL, 443)) { ok = false; break; }
         if (i == 0 && !warp_wait(BAR(acc_free), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_TMEM_EMPTY, 444)) { ok = false; break; }
         tc_fence_after();
-        mma_from_tmem(t_dv, t_s, sb + kKvDo + ds * kTileBytes, i != 0, BAR(do_empty) + 8 * ds);
+        mma_from_tmem(t_dv, t_s, sb + kKvDo + ds * kKvStage, i != 0, BAR(do_empty) + 8 * ds);
         if (more && !issue_s(n + 1)) { ok = false; break; }
         if (!warp_wait(BAR(ds_full), n & 1u, p.status, ST_TIMEOUT_FULL, 445)) { ok = false; break; }
         tc_fence_after();
-        mma_from_tmem(t_dk, t_dp, sb + kKvQ + qs * kTileBytes, i != 0, BAR(q_empty) + 8 * qs);
+        mma_from_tmem(t_dk, t_dp, sb + kKvQ + qs * kKvStage, i != 0, BAR(q_empty) + 8 * qs);
         if (more && !issue_dp(n + 1)) { ok = false; break; }
+        if (i + 2 == steps) warp_commit(BAR(kv_empty));      // the last products that read K and V are issued: both may be replaced
       }
       if (!ok) break;
-      warp_commit(BAR(kv_empty));
       warp_commit(BAR(acc_full));
       ++it;
     }
@@ -687,51 +734,47 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     uint32_t it = 0, n = 0;
     bool ok = true;
     KvWalk walk;
-    for (bool go = walk.begin(p, items); go && ok; go = walk.next(p, items)) {
+    for (bool go = walk.begin(p, items); go && ok; go = walk.next(p)) {
       const KvItem& t = walk.t;
       const int k_pos = t.k0 + row;
       int qt = walk.i0 % t.tiles;
       for (int i = walk.i0; i < walk.i1; ++i, ++n) {
         const int q0 = (t.first + qt) * kBlk + half * 64;
         if (++qt == t.tiles) qt = 0;
-        const uint32_t ss = n % kKvStatStages;
-        const float4* stat = reinterpret_cast<const float4*>(smem + kKvStat + ss * 1024 + half * 256);
         // visible queries of this key: [lo, hi) of the 64
         const int lo = k_pos - q0;
         const int hi = min(p.seq - q0, p.window > 0 ? min(lo, 64) + p.window : 64);
         const bool masked = __any_sync(kFullMask, lo > 0 || hi < 64);
-        if (!warp_wait(BAR(stat_full) + 8 * ss, (n / kKvStatStages) & 1u, p.status, ST_TIMEOUT_FULL, 450)) { ok = false; break; }
+        const uint32_t qs = n % kKvQStages;
+        const float4* lse2 = reinterpret_cast<const float4*>(smem + kKvQ + qs * kKvStage + kTileBytes + half * 256);
+        if (kCap && !warp_wait(BAR(q_full) + 8 * qs, (n / kKvQStages) & 1u, p.status, ST_TIMEOUT_FULL, 450)) { ok = false; break; }
         if (!warp_wait(BAR(s_full), n & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 451)) { ok = false; break; }
         tc_fence_after();
         Pair pr[32];
         uint32_t v[32], u[32], pk[32];
         // one branch per tile: the tests of a masked tile cost as much as the arithmetic
+        auto raw = [&](int i) { return i < 16 ? make_pair(v[(2 * i) & 31], v[(2 * i + 1) & 31]) : make_pair(u[(2 * i) & 31], u[(2 * i + 1) & 31]); };
         auto probabilities = [&](auto m) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float4 l = stat[i >> 1];
-#pragma unroll
-            for (int e = i; e < i + 2; ++e) {
-              Pair slope;
-              pr[e] = probability<kCap>(e < 16 ? make_pair(v[(2 * e) & 31], v[(2 * e + 1) & 31]) : make_pair(u[(2 * e) & 31], u[(2 * e + 1) & 31]),
-                                        e == i ? make_pair(l.x, l.y) : make_pair(l.z, l.w), p, slope);
-              if (decltype(m)::value) pr[e] = keep_range(pr[e], 2 * e, lo, hi);
-              pk[e] = pack_bf16(pr[e]);
-              if (kCap) pr[e] = mul2(pr[e], slope);
+          for (int i = 0; i < 32; ++i) {
+            Pair slope;
+            if (kCap) {
+              const float4 l = lse2[i >> 1];
+              pr[i] = probability<true>(raw(i), i & 1 ? make_pair(l.z, l.w) : make_pair(l.x, l.y), p, slope);
+            } else {
+              pr[i] = exp2_pair(mul2(raw(i), make_pair(p.scale_log2, p.scale_log2)));     // the log-sum-exp is in S already
             }
+            if (decltype(m)::value) pr[i] = keep_range(pr[i], 2 * i, lo, hi);
+            pk[i] = pack_bf16(pr[i]);
+            if (kCap) pr[i] = mul2(pr[i], slope);
           }
         };
         auto gradients = [&](auto m) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float4 l = stat[32 + (i >> 1)];
-#pragma unroll
-            for (int e = i; e < i + 2; ++e) {
-              const Pair dp = e < 16 ? make_pair(v[(2 * e) & 31], v[(2 * e + 1) & 31]) : make_pair(u[(2 * e) & 31], u[(2 * e + 1) & 31]);
-              Pair d = mul2(pr[e], add2(dp, e == i ? make_pair(l.x, l.y) : make_pair(l.z, l.w)));
-              if (decltype(m)::value) d = keep_range(d, 2 * e, lo, hi);
-              pk[e] = pack_bf16(d);
-            }
+          for (int i = 0; i < 32; ++i) {
+            Pair d = mul2(pr[i], raw(i));                                                 // and delta in dP
+            if (decltype(m)::value) d = keep_range(d, 2 * i, lo, hi);
+            pk[i] = pack_bf16(d);
           }
         };
         tc_ld_32x32b_x32(s_addr, v);
@@ -754,7 +797,6 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tc_wait_st();
         tc_fence_before();
         warp_arrive(BAR(ds_full));
-        warp_arrive(BAR(stat_empty) + 8 * ss);
       }
       if (!ok) break;
       if (!warp_wait(BAR(acc_full), it & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 453)) { ok = false; break; }
@@ -764,14 +806,16 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       tc_ld_32x32b_x32(t_dv + lane_addr + half * 64 + 32, b);
       tc_wait_ld();
       if (walk.i0 == 0 && walk.i1 == t.n) {
-        const size_t at = ((static_cast<size_t>(t.b) * p.seq + k_pos) * p.kv_heads + t.h) * kD + half * 64;
-        if (k_pos < p.seq) store_half_row(a, b, 1.0f, p.dv + at);
+        const int row0 = t.k0 + quad * 32;
+        const size_t at = ((static_cast<size_t>(t.b) * p.seq + row0) * p.kv_heads + t.h) * kD + half * 64;
+        const int64_t stride = static_cast<int64_t>(p.kv_heads) * kD;
+        store_half_rows(a, b, 1.0f, p.dv + at, stride, p.seq - row0);
         tc_ld_32x32b_x32(t_dk + lane_addr + half * 64, a);
         tc_ld_32x32b_x32(t_dk + lane_addr + half * 64 + 32, b);
         tc_wait_ld();
         tc_fence_before();
         warp_arrive(BAR(acc_free));
-        if (k_pos < p.seq) store_half_row(a, b, p.scale, p.dk + at);
+        store_half_rows(a, b, p.scale, p.dk + at, stride, p.seq - row0);
       } else {
         // part of a tile: fp32 sums for the joining kernel, 4 columns of all rows together
         float4* part = p.partial + (2 * static_cast<size_t>(blockIdx.x) + (walk.i0 == 0 ? 1 : 0)) * kPartVecs + half * 16 * kBlk + row;
@@ -800,14 +844,16 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 __global__ void __launch_bounds__(256)
 attention_bwd_join_kernel(const AttnBwdParams p) {
   const int c = blockIdx.x + 1;
-  int w, step;
-  const int64_t at = run_begin(p, c);
-  locate(p, at, w, step);
-  const int64_t begin = at - step;
-  if (step == 0 || run_begin(p, c - 1) > begin) return;      // no cut, or not the tile's first
+  int w, step, w2, step2;
+  run_begin(p, c, w, step);
+  run_begin(p, c - 1, w2, step2);
+  if (step == 0 || (w2 == w && step2 > 0)) return;           // no cut, or not the tile's first
   const KvItem t = kv_item(p, w);
   int last = c;                                              // the last run with steps of this tile
-  while (last + 1 < p.parts && run_begin(p, last + 1) < begin + t.n) ++last;
+  for (;; ++last) {
+    run_begin(p, last + 1, w2, step2);
+    if (w2 != w) break;
+  }
   const int row = threadIdx.x & (kBlk - 1);
   if (t.k0 + row >= p.seq) return;
   // 64 column groups of 4 (dV, dK) over 8 blocks and two halves of the CTA: 4 a thread, stored in pairs
@@ -846,9 +892,9 @@ KvPlan kv_plan(int batch, int seq, int kv_heads, int group, int window) {
   const int tiles = (seq + kBlk - 1) / kBlk;
   const int64_t bh = static_cast<int64_t>(batch) * kv_heads;
   KvPlan plan = {0, 0};
-  for (int kb = 0; kb < tiles; ++kb) plan.steps += kv_query_tiles(tiles, window, kb);
-  plan.steps *= bh * group;
-  const int64_t items = tiles * bh, longest = static_cast<int64_t>(kv_query_tiles(tiles, window, 0)) * group;
+  for (int kb = 0; kb < tiles; ++kb) plan.steps += kv_query_tiles(tiles, window, kb) * group + kTileSteps;
+  plan.steps *= bh;
+  const int64_t items = tiles * bh, longest = static_cast<int64_t>(kv_query_tiles(tiles, window, 0)) * group + kTileSteps;
   const int64_t even = plan.steps / kBwdRuns, waves = (items + kBwdRuns - 1) / kBwdRuns;
   int64_t whole = even + longest / 8;
   if (whole < longest) whole = longest;
@@ -887,7 +933,7 @@ bool encode_sequences(CUtensorMap* map, const void* base, uint64_t batch, uint64
 size_t attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv_heads, int window) {
   const size_t rows = static_cast<size_t>(batch) * q_heads * ((static_cast<size_t>(seq) + kBlk - 1) / kBlk * kBlk);
   const KvPlan plan = kv_plan(batch, seq, kv_heads, q_heads / kv_heads, window < seq ? window : 0);
-  return kBwdStatusBytes + 2 * rows * sizeof(float) + static_cast<size_t>(plan.parts) * 2 * kPartVecs * sizeof(float4);
+  return kBwdStatusBytes + 2 * rows * 32 + static_cast<size_t>(plan.parts) * 2 * kPartVecs * sizeof(float4);
 }
 
 cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream) {
@@ -913,14 +959,15 @@ cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream) {
   p.group = a.q_heads / a.kv_heads;
   p.window = a.window < a.seq ? a.window : 0;     // a window no shorter than the sequence hides nothing
   // the workspace: a status record for callers without one, the row constants, the parts of cut tiles
-  p.lse2 = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kBwdStatusBytes);
-  p.delta = p.lse2 + static_cast<int64_t>(a.batch) * a.q_heads * p.seq_pad;
-  p.partial = reinterpret_cast<float4*>(p.delta + static_cast<int64_t>(a.batch) * a.q_heads * p.seq_pad);
+  p.lse2 = static_cast<uint8_t*>(a.workspace) + kBwdStatusBytes;
+  p.delta = p.lse2 + static_cast<int64_t>(a.batch) * a.q_heads * p.seq_pad * 32;
+  p.partial = reinterpret_cast<float4*>(p.delta + static_cast<int64_t>(a.batch) * a.q_heads * p.seq_pad * 32);
   const KvPlan plan = kv_plan(a.batch, a.seq, a.kv_heads, p.group, p.window);
   p.parts = plan.parts;
   p.steps = plan.steps;
   p.scale = a.scale;
   p.scale_log2 = a.scale * kLog2e;
+  p.inv_scale_log2 = 1.0f / p.scale_log2;
   const bool cap = a.softcap > 0.0f;
   p.cap_in = cap ? 2.0f * kLog2e * a.scale / a.softcap : 0.0f;
   p.cap_out = a.softcap * kLog2e;

@@ -11,17 +11,20 @@ struct AttnBwdParams {
   const __nv_bfloat16* out;
   const __nv_bfloat16* d_out;
   const float* lse;          // [batch * q_heads, seq], natural log
-  float* lse2;               // [batch * q_heads, seq_pad]: base 2 and negated, -inf where a row has no probabilities
-  float* delta;              // [batch * q_heads, seq_pad], negated
+  // Left by the first kernel for the second, per 128-row tile of a query head: -delta, and the log-sum-exp as it is
+  // added to S, as tiles of constants (32 bytes a row); with a soft cap the latter as fp32 in base 2, negated.
+  // -inf where a row has no probabilities.
+  uint8_t* lse2;
+  uint8_t* delta;
   __nv_bfloat16* dq;
   __nv_bfloat16* dk;
   __nv_bfloat16* dv;
   int batch, seq, tiles, q_heads, kv_heads, group;
   int64_t seq_pad;           // tiles * 128
   int window;                // 0 = none
-  float scale, scale_log2;
+  float scale, scale_log2, inv_scale_log2;
   float cap_in, cap_out;     // soft cap: y = cap_out * tanh in base 2, 2 log2(e) * scale / cap on the way in
-  // dK, dV: runs of steps (0: whole tiles to CTAs) and the steps in all; two slots of fp32 sums a run
+  // dK, dV: runs of steps (0: whole tiles to CTAs), the length of all tiles in steps, two slots of fp32 sums a run
   int parts;
   int64_t steps;
   float4* partial;
