@@ -111,28 +111,28 @@ def attention_bwd(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
     gradient of `out`: (dq, dk, dv), bf16 like q, k, v. Any sequence length; dk and dv are summed over the query heads of their
     group. The same inputs give the same bits. `check` synchronises and raises on a device-side failure; under stream capture,
     or in a loop that checks once, pass check=False and a `status` of your own."""
-    B, S, Hq, d = q.shape if q.dim() == 4 else (0, 0, 0, 0)
-    Hkv = k.shape[2] if k.dim() == 4 else 0
-    if d != D or k.shape != (B, S, Hkv, D) or v.shape != k.shape or out.shape != q.shape or d_out.shape != q.shape:
+    q_shape, kv_shape, dev = q.shape, k.shape, q.device
+    if len(q_shape) != 4 or len(kv_shape) != 4 or q_shape[3] != D or kv_shape[3] != D or kv_shape[:2] != q_shape[:2] or \
+            v.shape != kv_shape or out.shape != q_shape or d_out.shape != q_shape:
         raise ValueError("attention_bwd wants q, out, d_out [B, S, Hq, 128] and k, v [B, S, Hkv, 128]")
-    if Hkv == 0 or Hq % Hkv:
+    B, S, Hq, _ = q_shape
+    Hkv = kv_shape[2]
+    if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError("the query heads must be a multiple of the KV heads")
-    if lse.shape != (B * Hq, S) or lse.dtype != torch.float32:
-        raise ValueError("lse is f32 [B * Hq, S], as attention_fwd returns it")
+    if lse.shape != (B * Hq, S) or lse.dtype is not torch.float32 or lse.device != dev:
+        raise ValueError("lse is f32 [B * Hq, S] on the same device, as attention_fwd returns it")
     for t in (d_out, q, k, v, out):
-        if t.dtype != torch.bfloat16 or not t.is_cuda or t.device != q.device:
+        if t.dtype is not torch.bfloat16 or t.device != dev or dev.type != "cuda":
             raise ValueError("attention_bwd wants bf16 CUDA tensors on one device")
-    if lse.device != q.device:
-        raise ValueError("lse lies on another device")
     if window < 0 or not softcap >= 0.0:
         raise ValueError("window and softcap are 0 (off) or positive")
     with device_of(q):
-        d_out, q, k, v, out, lse = (dense(t) for t in (d_out, q, k, v, out, lse))
+        d_out, q, k, v, out, lse = dense(d_out), dense(q), dense(k), dense(v), dense(out), dense(lse)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         if B == 0 or S == 0:
             return dq, dk, dv
         nbytes = _lib.load().plb_attention_bwd_workspace_bytes(B, S, Hq, Hkv, int(window))
-        workspace = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         if status is None and check:
             status = DeviceStatus(q.device)
         _lib.call("plb_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), d_out.data_ptr(), lse.data_ptr(),

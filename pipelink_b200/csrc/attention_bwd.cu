@@ -20,6 +20,7 @@
 // next sequence's, and their probabilities are forced to 0 (log-sum-exp +inf), so any length works.
 #include <math.h>
 
+#include <atomic>
 #include <cstddef>
 
 #include "attention_bwd.h"
@@ -61,7 +62,7 @@ struct DqBars {
 };
 struct KvBars {
   uint64_t kv_full, kv_empty, q_full[kKvQStages], q_empty[kKvQStages], do_full[kKvDoStages], do_empty[kKvDoStages];
-  uint64_t s_full, p_full, dp_full, ds_full, acc_full, acc_free, drain;
+  uint64_t s_full, p_full[2], dp_full, ds_full, acc_full, acc_free, drain;
   uint32_t tmem_base, pad;
 };
 static_assert(sizeof(DqBars) <= 256 && sizeof(KvBars) <= 256, "barrier block");
@@ -102,45 +103,33 @@ __device__ __forceinline__ KvItem kv_item(const AttnBwdParams& p, int w) {
   t.n = t.tiles * p.group;
   return t;
 }
-// The key tiles' steps (a step: one query tile of one head) in one line, heaviest tiles first, cut into p.parts runs
-// of equal time, where a tile counts kTileSteps more than it has, for its loads and stores: where run r begins, as a
-// tile and a step of it.
+// The key tiles' steps (a step: one query tile of one head) in one line, heaviest tiles first, cut into equal runs,
+// where a tile counts kTileSteps more than it has, for its loads and stores: run r begins at step[r] of tile w[r].
 constexpr int kTileSteps = 2;
-__device__ __forceinline__ void run_begin(const AttnBwdParams& p, int r, int& w, int& step) {
-  const int bh = p.batch * p.kv_heads;
-  int64_t at = p.steps * r / p.parts;
-  for (int kb = 0; kb < p.tiles; ++kb) {
-    const int n = kv_query_tiles(p.tiles, p.window, kb) * p.group + kTileSteps;
-    if (at < static_cast<int64_t>(n) * bh) {
-      const int i = static_cast<int>(at / n);
-      w = kb * bh + i;
-      step = max(0, static_cast<int>(at - static_cast<int64_t>(i) * n) - kTileSteps);
-      return;
-    }
-    at -= static_cast<int64_t>(n) * bh;
-  }
-  w = p.tiles * bh;
-  step = 0;
-}
-// What a CTA works through: whole tiles (parts 0, the list walked forth and back) or its run, steps [i0, i1) of tile w.
+struct Runs { int count, w[kBwdRuns + 1], step[kBwdRuns + 1]; };
+// What a CTA works through: whole tiles (no runs, the list walked forth and back) or its run, steps [i0, i1) of tile w.
 struct KvWalk {
   int w, i0, i1, wave, end_w, end_step;
   KvItem t;
-  __device__ __forceinline__ bool begin(const AttnBwdParams& p, int items) {
+  bool whole;
+  __device__ __forceinline__ bool begin(const AttnBwdParams& p, const Runs& runs, int items) {
     wave = 0;
     i0 = 0;
     end_w = items;
     end_step = 0;
-    if (p.parts > 0) {
-      run_begin(p, blockIdx.x, w, i0);
-      run_begin(p, blockIdx.x + 1, end_w, end_step);
+    whole = runs.count == 0;
+    if (!whole) {
+      w = runs.w[blockIdx.x];
+      i0 = runs.step[blockIdx.x];
+      end_w = runs.w[blockIdx.x + 1];
+      end_step = runs.step[blockIdx.x + 1];
     } else {
       w = snake(0);
     }
     return set(p);
   }
   __device__ __forceinline__ bool next(const AttnBwdParams& p) {
-    if (p.parts > 0) {
+    if (!whole) {
       ++w;
       i0 = 0;
     } else {
@@ -203,13 +192,15 @@ __device__ __forceinline__ void mma_tiles(uint32_t d, uint32_t a, uint32_t b, ui
   __syncwarp();
 }
 // D += A B with A bf16 in tensor memory (its two 64-column halves at a and a + 64) and B's rows along the contraction.
-__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint32_t b, bool accumulate, uint32_t bar) {
+// Steps k0, k0 + 1 of each half if `part`, else all eight; the barrier may be 0.
+__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint32_t b, bool accumulate, uint32_t bar, bool part = false, int k0 = 0) {
   const uint64_t bd = smem_desc(b, kDescVMn);
   if (elect_one_sync()) {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      tc_mma_f16_ts(d, a + (k >> 2) * 64 + (k & 3) * 8, bd + ((k * 2048) >> 4), kIdescPV, k != 0 || accumulate ? 1u : 0u);
-    tc_commit(bar);
+      if (!part || (k & 2) == k0)
+        tc_mma_f16_ts(d, a + (k >> 2) * 64 + (k & 3) * 8, bd + ((k * 2048) >> 4), kIdescPV, k != k0 || accumulate ? 1u : 0u);
+    if (bar != 0) tc_commit(bar);
   }
   __syncwarp();
 }
@@ -602,7 +593,7 @@ template <bool kCap>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
                           const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                          const AttnBwdParams p) {
+                          const __grid_constant__ AttnBwdParams p, const __grid_constant__ Runs runs) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sb = smem_u32(smem);
   if ((sb & 1023u) != 0) {          // the swizzle pattern repeats every 1024 bytes
@@ -619,6 +610,7 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     for (int s = 0; s < kKvDoStages; ++s) { mbar_init(BAR(do_full) + 8 * s, 1); mbar_init(BAR(do_empty) + 8 * s, 1); }
     mbar_init(BAR(s_full), 1);
     mbar_init(BAR(p_full), kComputeWarps);
+    mbar_init(BAR(p_full) + 8, kComputeWarps);
     mbar_init(BAR(dp_full), 1);
     mbar_init(BAR(ds_full), kComputeWarps);
     mbar_init(BAR(acc_full), 1);
@@ -647,7 +639,7 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     uint32_t it = 0, n = 0;
     bool ok = true;
     KvWalk walk;
-    for (bool go = walk.begin(p, items); go && ok; go = walk.next(p)) {
+    for (bool go = walk.begin(p, runs, items); go && ok; go = walk.next(p)) {
       const KvItem& t = walk.t;
       if (!warp_wait(BAR(kv_empty), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_EMPTY, 430)) { ok = false; break; }
       if (elect_one_sync()) {
@@ -702,7 +694,7 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       return true;
     };
     KvWalk walk;
-    for (bool go = walk.begin(p, items); go && ok; go = walk.next(p)) {
+    for (bool go = walk.begin(p, runs, items); go && ok; go = walk.next(p)) {
       const int steps = __shfl_sync(kFullMask, walk.i1 - walk.i0, 0);
       if (!warp_wait(BAR(kv_full), it & 1u, p.status, ST_TIMEOUT_FULL, 442)) { ok = false; break; }
       tc_fence_after();
@@ -714,7 +706,11 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         if (!warp_wait(BAR(p_full), n & 1u, p.status, ST_TIMEOUT_FULL, 443)) { ok = false; break; }
         if (i == 0 && !warp_wait(BAR(acc_free), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_TMEM_EMPTY, 444)) { ok = false; break; }
         tc_fence_after();
-        mma_from_tmem(t_dv, t_s, sb + kKvDo + ds * kKvStage, i != 0, BAR(do_empty) + 8 * ds);
+        // dV's product starts on the half of P that is ready first
+        mma_from_tmem(t_dv, t_s, sb + kKvDo + ds * kKvStage, i != 0, 0, true, 0);
+        if (!warp_wait(BAR(p_full) + 8, n & 1u, p.status, ST_TIMEOUT_FULL, 446)) { ok = false; break; }
+        tc_fence_after();
+        mma_from_tmem(t_dv, t_s, sb + kKvDo + ds * kKvStage, true, BAR(do_empty) + 8 * ds, true, 2);
         if (more && !issue_s(n + 1)) { ok = false; break; }
         if (!warp_wait(BAR(ds_full), n & 1u, p.status, ST_TIMEOUT_FULL, 445)) { ok = false; break; }
         tc_fence_after();
@@ -734,7 +730,7 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     uint32_t it = 0, n = 0;
     bool ok = true;
     KvWalk walk;
-    for (bool go = walk.begin(p, items); go && ok; go = walk.next(p)) {
+    for (bool go = walk.begin(p, runs, items); go && ok; go = walk.next(p)) {
       const KvItem& t = walk.t;
       const int k_pos = t.k0 + row;
       int qt = walk.i0 % t.tiles;
@@ -754,9 +750,9 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         uint32_t v[32], u[32], pk[32];
         // one branch per tile: the tests of a masked tile cost as much as the arithmetic
         auto raw = [&](int i) { return i < 16 ? make_pair(v[(2 * i) & 31], v[(2 * i + 1) & 31]) : make_pair(u[(2 * i) & 31], u[(2 * i + 1) & 31]); };
-        auto probabilities = [&](auto m) {
+        auto probabilities = [&](auto m, int from) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = from; i < from + 16; ++i) {
             Pair slope;
             if (kCap) {
               const float4 l = lse2[i >> 1];
@@ -780,12 +776,18 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tc_ld_32x32b_x32(s_addr, v);
         tc_ld_32x32b_x32(s_addr + 32, u);
         tc_wait_ld();
-        if (masked) probabilities(TrueTag{});
-        else probabilities(FalseTag{});
-        tc_st_32x32b_x32(s_addr, pk);
-        tc_wait_st();
-        tc_fence_before();
-        warp_arrive(BAR(p_full));
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (masked) probabilities(TrueTag{}, 16 * c);
+          else probabilities(FalseTag{}, 16 * c);
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = pk[16 * c + i];
+          tc_st_32x32b_x16(s_addr + 16 * c, w);
+          tc_wait_st();
+          tc_fence_before();
+          warp_arrive(BAR(p_full) + 8 * c);
+        }
         if (!warp_wait(BAR(dp_full), n & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 452)) { ok = false; break; }
         tc_fence_after();
         tc_ld_32x32b_x32(dp_addr, v);
@@ -842,18 +844,12 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 // Tiles that more than one run worked on: block (c, y) takes the tile whose first cut is where run c begins, and an
 // eighth of its columns; the parts are added in the order of their runs.
 __global__ void __launch_bounds__(256)
-attention_bwd_join_kernel(const AttnBwdParams p) {
-  const int c = blockIdx.x + 1;
-  int w, step, w2, step2;
-  run_begin(p, c, w, step);
-  run_begin(p, c - 1, w2, step2);
-  if (step == 0 || (w2 == w && step2 > 0)) return;           // no cut, or not the tile's first
+attention_bwd_join_kernel(const __grid_constant__ AttnBwdParams p, const __grid_constant__ Runs runs) {
+  const int c = blockIdx.x + 1, w = runs.w[c];
+  if (runs.step[c] == 0 || (runs.w[c - 1] == w && runs.step[c - 1] > 0)) return;     // no cut, or not the tile's first
   const KvItem t = kv_item(p, w);
   int last = c;                                              // the last run with steps of this tile
-  for (;; ++last) {
-    run_begin(p, last + 1, w2, step2);
-    if (w2 != w) break;
-  }
+  while (runs.w[last + 1] == w) ++last;
   const int row = threadIdx.x & (kBlk - 1);
   if (t.k0 + row >= p.seq) return;
   // 64 column groups of 4 (dV, dK) over 8 blocks and two halves of the CTA: 4 a thread, stored in pairs
@@ -887,21 +883,37 @@ attention_bwd_join_kernel(const AttnBwdParams p) {
 // tiles differ in length by their number) or the last wave is short; equal runs of steps leave none idle and cost
 // the parts' fp32 sums and the joining kernel, about ten steps' time. Measured at 2048 positions, 32 / 8 heads:
 // kPlanNote.
-struct KvPlan { int parts; int64_t steps; };
-KvPlan kv_plan(int batch, int seq, int kv_heads, int group, int window) {
-  const int tiles = (seq + kBlk - 1) / kBlk;
-  const int64_t bh = static_cast<int64_t>(batch) * kv_heads;
-  KvPlan plan = {0, 0};
-  for (int kb = 0; kb < tiles; ++kb) plan.steps += kv_query_tiles(tiles, window, kb) * group + kTileSteps;
-  plan.steps *= bh;
-  const int64_t items = tiles * bh, longest = static_cast<int64_t>(kv_query_tiles(tiles, window, 0)) * group + kTileSteps;
-  const int64_t even = plan.steps / kBwdRuns, waves = (items + kBwdRuns - 1) / kBwdRuns;
+Runs kv_runs(int batch, int seq, int kv_heads, int group, int window) {
+  const int tiles = (seq + kBlk - 1) / kBlk, bh = batch * kv_heads;
+  auto length = [&](int kb) { return static_cast<int64_t>(kv_query_tiles(tiles, window, kb)) * group + kTileSteps; };
+  int64_t steps = 0;
+  for (int kb = 0; kb < tiles; ++kb) steps += length(kb);
+  steps *= bh;
+  Runs runs;
+  runs.count = 0;
+  const int64_t items = static_cast<int64_t>(tiles) * bh, longest = length(0);
+  const int64_t even = steps / kBwdRuns, waves = (items + kBwdRuns - 1) / kBwdRuns;
   int64_t whole = even + longest / 8;
   if (whole < longest) whole = longest;
-  if (whole < waves * plan.steps / items) whole = waves * plan.steps / items;
-  if (whole > even + 10) plan.parts = static_cast<int>(plan.steps / 8 < kBwdRuns ? plan.steps / 8 : kBwdRuns);
-  if (plan.parts < 2) plan.parts = 0;
-  return plan;
+  if (whole < waves * steps / items) whole = waves * steps / items;
+  if (whole <= even + 10 || steps < 16) return runs;
+  runs.count = static_cast<int>(steps / 8 < kBwdRuns ? steps / 8 : kBwdRuns);
+  int64_t before = 0;                                        // where tile row kb begins
+  int r = 0;
+  for (int kb = 0; kb < tiles; ++kb) {
+    const int64_t n = length(kb);
+    for (; r < runs.count; ++r) {
+      const int64_t at = steps * r / runs.count - before;
+      if (at >= n * bh) break;
+      const int64_t step = at % n - kTileSteps;
+      runs.w[r] = kb * bh + static_cast<int>(at / n);
+      runs.step[r] = step > 0 ? static_cast<int>(step) : 0;
+    }
+    before += n * bh;
+  }
+  runs.w[r] = static_cast<int>(items);
+  runs.step[r] = 0;
+  return runs;
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -932,8 +944,8 @@ bool encode_sequences(CUtensorMap* map, const void* base, uint64_t batch, uint64
 
 size_t attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv_heads, int window) {
   const size_t rows = static_cast<size_t>(batch) * q_heads * ((static_cast<size_t>(seq) + kBlk - 1) / kBlk * kBlk);
-  const KvPlan plan = kv_plan(batch, seq, kv_heads, q_heads / kv_heads, window < seq ? window : 0);
-  return kBwdStatusBytes + 2 * rows * 32 + static_cast<size_t>(plan.parts) * 2 * kPartVecs * sizeof(float4);
+  const Runs runs = kv_runs(batch, seq, kv_heads, q_heads / kv_heads, window < seq ? window : 0);
+  return kBwdStatusBytes + 2 * rows * 32 + static_cast<size_t>(runs.count) * 2 * kPartVecs * sizeof(float4);
 }
 
 cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream) {
@@ -962,9 +974,7 @@ cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream) {
   p.lse2 = static_cast<uint8_t*>(a.workspace) + kBwdStatusBytes;
   p.delta = p.lse2 + static_cast<int64_t>(a.batch) * a.q_heads * p.seq_pad * 32;
   p.partial = reinterpret_cast<float4*>(p.delta + static_cast<int64_t>(a.batch) * a.q_heads * p.seq_pad * 32);
-  const KvPlan plan = kv_plan(a.batch, a.seq, a.kv_heads, p.group, p.window);
-  p.parts = plan.parts;
-  p.steps = plan.steps;
+  const Runs runs = kv_runs(a.batch, a.seq, a.kv_heads, p.group, p.window);
   p.scale = a.scale;
   p.scale_log2 = a.scale * kLog2e;
   p.inv_scale_log2 = 1.0f / p.scale_log2;
@@ -981,18 +991,26 @@ cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream) {
   const int64_t kv_items = static_cast<int64_t>(p.tiles) * a.batch * a.kv_heads;
   auto dq = cap ? attention_bwd_dq_kernel<true> : attention_bwd_dq_kernel<false>;
   auto dkdv = cap ? attention_bwd_dkdv_kernel<true> : attention_bwd_dkdv_kernel<false>;
-  cudaError_t err = cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, kDqSmem);
+  // shared-memory limits of the two kernels, once per device
+  static std::atomic<bool> ready[2][64];
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
   if (err != cudaSuccess) return err;
-  err = cudaFuncSetAttribute(dkdv, cudaFuncAttributeMaxDynamicSharedMemorySize, kKvSmem);
-  if (err != cudaSuccess) return err;
+  if (device >= 64 || !ready[cap][device].load(std::memory_order_relaxed)) {
+    err = cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, kDqSmem);
+    if (err != cudaSuccess) return err;
+    err = cudaFuncSetAttribute(dkdv, cudaFuncAttributeMaxDynamicSharedMemorySize, kKvSmem);
+    if (err != cudaSuccess) return err;
+    if (device < 64) ready[cap][device].store(true, std::memory_order_relaxed);
+  }
   dq<<<static_cast<int>(q_items < a.num_sms ? q_items : a.num_sms), kBwdThreads, kDqSmem, stream>>>(mq, mdo, mk, mv, p);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
-  const int grid = p.parts > 0 ? p.parts : static_cast<int>(kv_items < a.num_sms ? kv_items : a.num_sms);
-  dkdv<<<grid, kBwdThreads, kKvSmem, stream>>>(mq, mdo, mk, mv, p);
+  const int grid = runs.count > 0 ? runs.count : static_cast<int>(kv_items < a.num_sms ? kv_items : a.num_sms);
+  dkdv<<<grid, kBwdThreads, kKvSmem, stream>>>(mq, mdo, mk, mv, p, runs);
   err = cudaGetLastError();
-  if (err != cudaSuccess || p.parts == 0) return err;
-  attention_bwd_join_kernel<<<dim3(p.parts - 1, 8), 256, 0, stream>>>(p);
+  if (err != cudaSuccess || runs.count < 2) return err;
+  attention_bwd_join_kernel<<<dim3(runs.count - 1, 8), 256, 0, stream>>>(p, runs);
   return cudaGetLastError();
 }
 

@@ -24,10 +24,7 @@ struct AttnBwdParams {
   int window;                // 0 = none
   float scale, scale_log2, inv_scale_log2;
   float cap_in, cap_out;     // soft cap: y = cap_out * tanh in base 2, 2 log2(e) * scale / cap on the way in
-  // dK, dV: runs of steps (0: whole tiles to CTAs), the length of all tiles in steps, two slots of fp32 sums a run
-  int parts;
-  int64_t steps;
-  float4* partial;
+  float4* partial;           // two slots of fp32 sums of dK and dV a run
   Status* status;
 };
 

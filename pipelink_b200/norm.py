@@ -6,7 +6,7 @@ launch; ``rmsnorm_bwd`` returns the gradient that both summands share and the we
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -14,8 +14,7 @@ from . import _lib
 from .mok import _ptr, _stream, dense, device_of, rows_of
 
 
-@dataclass(frozen=True)
-class Normed:
+class Normed(NamedTuple):
     hidden: torch.Tensor        # bf16, x + residual (x itself without a residual): the stream, and what the backward pass reads
     rstd: torch.Tensor          # f32 [rows]
     y: torch.Tensor | None      # bf16, like x
@@ -23,53 +22,57 @@ class Normed:
     sc: torch.Tensor | None     # u8 [that / 128, width / 128, 32, 16]
 
 
-def _check(name, t, like, shape):
-    if t.dtype != torch.bfloat16 or not t.is_cuda or t.device != like.device or t.shape != shape:
-        raise ValueError(f"{name} is a bf16 tensor of shape {tuple(shape)} on {like.device}")
+def _check(name, t, device, shape):
+    if t.dtype is not torch.bfloat16 or t.device != device or t.shape != shape or device.type != "cuda":
+        raise ValueError(f"{name} is a bf16 tensor of shape {tuple(shape)} on one CUDA device")
+
+
+def _check_into(into: Normed, residual, out, rows, width, padded, device):
+    for name, t, n, dtype in (("hidden", into.hidden if residual is not None else None, rows * width, torch.bfloat16),
+                              ("rstd", into.rstd, rows, torch.float32), ("y", into.y, rows * width, torch.bfloat16),
+                              ("fp8", into.fp8, padded * width, torch.uint8), ("sc", into.sc, padded * width // 32, torch.uint8)):
+        if t is not None and (t.numel() != n or t.dtype != dtype or t.device != device or not t.is_contiguous()):
+            raise ValueError(f"into.{name} is a contiguous {dtype} tensor of {n} elements on {device}")
+    if into.rstd is None or (into.y is None) != (out == "mxfp8") or (into.fp8 is None) != (out == "bf16") or \
+            (into.sc is None) != (out == "bf16") or (residual is not None and into.hidden is None):
+        raise ValueError("into holds the outputs that were asked for, and no others")
 
 
 def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-5,
                 out: str = "bf16", into: Normed | None = None) -> Normed:
     """x, residual bf16 [..., width], weight bf16 [width]. `out`: "bf16", "mxfp8" (width a multiple of 128) or "both".
     hidden = bf16(x + residual), y = bf16(hidden * rstd * weight). `into` gives the tensors to write (contiguous; those of
-    an earlier call of the same shape, or a session's buffers) instead of new ones."""
+    an earlier call of the same shape, or a session's buffers) instead of new ones; its hidden may be the residual itself."""
     if out not in ("bf16", "mxfp8", "both"):
         raise ValueError("out is 'bf16', 'mxfp8' or 'both'")
-    if x.dim() < 1 or x.shape[-1] < 1:
+    shape, dev = x.shape, x.device
+    width = shape[-1] if shape else 0
+    if width < 1:
         raise ValueError("x is [..., width]")
-    width = x.shape[-1]
-    _check("x", x, x, x.shape)
-    _check("weight", weight, x, (width,))
+    _check("x", x, dev, shape)
+    _check("weight", weight, dev, (width,))
     if residual is not None:
-        _check("residual", residual, x, x.shape)
+        _check("residual", residual, dev, shape)
     if not eps >= 0.0:
         raise ValueError("eps is not negative")
     if out != "bf16" and width % 128:
         raise ValueError("MXFP8 output wants a width that is a multiple of 128")
+    rows = x.numel() // width
+    padded = (rows + 127) // 128 * 128
     with device_of(x):
-        rows = x.numel() // width
         x2, ld_x = rows_of(x)
         r2, ld_r = rows_of(residual) if residual is not None else (None, 0)
         weight = dense(weight)
-        dev, padded = x.device, (rows + 127) // 128 * 128
         if into is None:
-            u8 = dict(dtype=torch.uint8, device=dev)
-            into = Normed(hidden=torch.empty(x.shape, dtype=torch.bfloat16, device=dev) if residual is not None else x,
-                          rstd=torch.empty(rows, dtype=torch.float32, device=dev),
-                          y=torch.empty(x.shape, dtype=torch.bfloat16, device=dev) if out != "mxfp8" else None,
-                          fp8=torch.empty((padded, width), **u8) if out != "bf16" else None,
-                          sc=torch.empty((padded // 128, width // 128, 32, 16), **u8) if out != "bf16" else None)
+            into = Normed(torch.empty(shape, dtype=torch.bfloat16, device=dev) if residual is not None else x,
+                          torch.empty(rows, dtype=torch.float32, device=dev),
+                          torch.empty(shape, dtype=torch.bfloat16, device=dev) if out != "mxfp8" else None,
+                          torch.empty((padded, width), dtype=torch.uint8, device=dev) if out != "bf16" else None,
+                          torch.empty((padded // 128, width // 128, 32, 16), dtype=torch.uint8, device=dev) if out != "bf16" else None)
         else:
-            for name, t, n, dtype in (("hidden", into.hidden if residual is not None else None, rows * width, torch.bfloat16),
-                                      ("rstd", into.rstd, rows, torch.float32), ("y", into.y, rows * width, torch.bfloat16),
-                                      ("fp8", into.fp8, padded * width, torch.uint8), ("sc", into.sc, padded * width // 32, torch.uint8)):
-                if t is not None and (t.numel() != n or t.dtype != dtype or t.device != dev or not t.is_contiguous()):
-                    raise ValueError(f"into.{name} is a contiguous {dtype} tensor of {n} elements on {dev}")
-            if into.rstd is None or (into.y is None) != (out == "mxfp8") or (into.fp8 is None) != (out == "bf16") or \
-                    (into.sc is None) != (out == "bf16") or (residual is not None and into.hidden is None):
-                raise ValueError("into holds the outputs that were asked for, and no others")
-        _lib.call("plb_rmsnorm_fwd", x2.data_ptr(), ld_x, _ptr(r2), ld_r, weight.data_ptr(), rows, width, float(eps),
-                  _ptr(into.hidden) if residual is not None else 0, into.rstd.data_ptr(), _ptr(into.y), _ptr(into.fp8),
+            _check_into(into, residual, out, rows, width, padded, dev)
+        _lib.call("plb_rmsnorm_fwd", x2.data_ptr(), ld_x, _ptr(r2), ld_r, weight.data_ptr(), rows, width, eps,
+                  into.hidden.data_ptr() if residual is not None else 0, into.rstd.data_ptr(), _ptr(into.y), _ptr(into.fp8),
                   _ptr(into.sc), _stream())
     return into
 
@@ -79,26 +82,27 @@ def rmsnorm_bwd(d_y: torch.Tensor, hidden: torch.Tensor, rstd: torch.Tensor, wei
     """Gradient of ``rmsnorm_fwd``: (d_x, d_weight). d_x (bf16, like hidden) is the gradient of x and of the residual alike,
     d_weight f32 [width]. `d_hidden` is the gradient that reaches the residual stream past the norm. An MXFP8 output has
     its bf16 value's gradient. The same inputs give the same bits."""
-    if hidden.dim() < 1 or hidden.shape[-1] < 1:
+    shape, dev = hidden.shape, hidden.device
+    width = shape[-1] if shape else 0
+    if width < 1:
         raise ValueError("hidden is [..., width]")
-    width = hidden.shape[-1]
     rows = hidden.numel() // width
-    _check("hidden", hidden, hidden, hidden.shape)
-    _check("d_y", d_y, hidden, hidden.shape)
-    _check("weight", weight, hidden, (width,))
+    _check("hidden", hidden, dev, shape)
+    _check("d_y", d_y, dev, shape)
+    _check("weight", weight, dev, (width,))
     if d_hidden is not None:
-        _check("d_hidden", d_hidden, hidden, hidden.shape)
-    if rstd.shape != (rows,) or rstd.dtype != torch.float32 or rstd.device != hidden.device:
+        _check("d_hidden", d_hidden, dev, shape)
+    if rstd.shape != (rows,) or rstd.dtype is not torch.float32 or rstd.device != dev:
         raise ValueError("rstd is f32 [rows], as rmsnorm_fwd returns it")
     with device_of(hidden):
         g2, ld_g = rows_of(d_y)
         h2, ld_h = rows_of(hidden)
         e2, ld_e = rows_of(d_hidden) if d_hidden is not None else (None, 0)
         rstd, weight = rstd.contiguous(), dense(weight)
-        d_x = torch.empty(hidden.shape, dtype=torch.bfloat16, device=hidden.device)
-        d_weight = torch.empty(width, dtype=torch.float32, device=hidden.device)
+        d_x = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        d_weight = torch.empty(width, dtype=torch.float32, device=dev)
         nbytes = _lib.load().plb_rmsnorm_bwd_workspace_bytes(rows, width)
-        workspace = torch.empty(nbytes // 4, dtype=torch.float32, device=hidden.device)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _lib.call("plb_rmsnorm_bwd", g2.data_ptr(), ld_g, h2.data_ptr(), ld_h, rstd.data_ptr(), weight.data_ptr(), _ptr(e2), ld_e,
                   rows, width, d_x.data_ptr(), d_weight.data_ptr(), workspace.data_ptr(), nbytes, _stream())
     return d_x, d_weight

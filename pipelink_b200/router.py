@@ -11,11 +11,12 @@ from . import _lib
 from .mok import _ptr, _stream, device_of, rows_of
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
+_DTYPES = (torch.float32, torch.bfloat16)
 MAX_EXPERTS, MAX_TOPK, MAX_GROUPS = 1024, 32, 32
 
 
 def _check(logits, topk, score):
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or not logits.is_cuda:
+    if logits.dim() != 2 or logits.dtype not in _DTYPES or not logits.is_cuda:
         raise ValueError("logits are a CUDA f32 or bf16 tensor [tokens, experts]")
     experts = logits.shape[1]
     if not 1 <= experts <= MAX_EXPERTS or not 1 <= topk <= min(MAX_TOPK, experts):
@@ -36,11 +37,12 @@ def route_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias:
     cannot tell apart are told apart. `into` gives the two contiguous tensors to write (a session's buffers)."""
     _check(logits, topk, score)
     tokens, experts = logits.shape
+    dev = logits.device
     if group_score not in ("top2", "max"):
         raise ValueError("group_score is 'top2' or 'max'")
     if not 1 <= groups <= MAX_GROUPS or experts % groups or not 1 <= topk_groups <= groups or topk > topk_groups * (experts // groups):
         raise ValueError(f"groups (at most {MAX_GROUPS}) divide the experts, and the kept ones hold at least topk experts")
-    if bias is not None and (bias.shape != (experts,) or bias.dtype != torch.float32 or bias.device != logits.device):
+    if bias is not None and (bias.shape != (experts,) or bias.dtype != torch.float32 or bias.device != dev):
         raise ValueError("bias is f32 [experts] on the logits' device")
     if scale != scale:
         raise ValueError("scale is a number")
@@ -48,12 +50,13 @@ def route_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias:
         x, ld = rows_of(logits)
         bias = bias.contiguous() if bias is not None else None
         if into is None:
-            into = (torch.empty((tokens, topk), dtype=torch.int32, device=logits.device),
-                    torch.empty((tokens, topk), dtype=torch.float32, device=logits.device))
-        chosen, weights = into
-        for t, dtype in ((chosen, torch.int32), (weights, torch.float32)):
-            if t.numel() != tokens * topk or t.dtype != dtype or t.device != logits.device or not t.is_contiguous():
-                raise ValueError("into holds contiguous i32 and f32 tensors of tokens * topk elements on the logits' device")
+            chosen = torch.empty((tokens, topk), dtype=torch.int32, device=dev)
+            weights = torch.empty((tokens, topk), dtype=torch.float32, device=dev)
+        else:
+            chosen, weights = into
+            for t, dtype in ((chosen, torch.int32), (weights, torch.float32)):
+                if t.numel() != tokens * topk or t.dtype is not dtype or t.device != dev or not t.is_contiguous():
+                    raise ValueError("into holds contiguous i32 and f32 tensors of tokens * topk elements on the logits' device")
         _lib.call("plb_route_topk", x.data_ptr(), ld, int(x.dtype == torch.bfloat16), _ptr(bias), tokens, experts, topk,
                   _SCORES[score], groups, topk_groups, int(group_score == "top2"), int(renormalize), float(scale), chosen.data_ptr(),
                   weights.data_ptr(), _stream())
@@ -66,17 +69,17 @@ def route_topk_bwd(d_weights: torch.Tensor, logits: torch.Tensor, experts: torch
     (bias and groups decide the choice alone and have no gradient)."""
     topk = experts.shape[1] if experts.dim() == 2 else 0
     _check(logits, topk, score)
-    tokens = logits.shape[0]
-    if experts.shape != (tokens, topk) or experts.dtype != torch.int32 or experts.device != logits.device:
+    tokens, dev = logits.shape[0], logits.device
+    if experts.shape != (tokens, topk) or experts.dtype is not torch.int32 or experts.device != dev:
         raise ValueError("experts are i32 [tokens, topk] on the logits' device")
-    if d_weights.shape != (tokens, topk) or d_weights.dtype != torch.float32 or d_weights.device != logits.device:
+    if d_weights.shape != (tokens, topk) or d_weights.dtype is not torch.float32 or d_weights.device != dev:
         raise ValueError("d_weights are f32 [tokens, topk] on the logits' device")
     if scale != scale:
         raise ValueError("scale is a number")
     with device_of(logits):
         x, ld = rows_of(logits)
         d_weights, experts = d_weights.contiguous(), experts.contiguous()
-        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         _lib.call("plb_route_topk_bwd", d_weights.data_ptr(), x.data_ptr(), ld, int(x.dtype == torch.bfloat16), experts.data_ptr(),
                   tokens, logits.shape[1], topk, _SCORES[score], int(renormalize), float(scale), d_logits.data_ptr(), _stream())
     return d_logits
