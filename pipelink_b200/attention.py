@@ -132,7 +132,7 @@ def attention_bwd(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
         if B == 0 or S == 0:
             return dq, dk, dv
         nbytes = _lib.load().plb_attention_bwd_workspace_bytes(B, S, Hq, Hkv, int(window))
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        workspace = q.new_empty(nbytes, dtype=torch.uint8)
         if status is None and check:
             status = DeviceStatus(q.device)
         _lib.call("plb_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), d_out.data_ptr(), lse.data_ptr(),

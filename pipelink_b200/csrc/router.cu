@@ -5,11 +5,13 @@
 //   the topk best c of the kept groups, ties to the lowest index; w = scale * s [/ sum of the chosen s]
 //   dS_j = scale / S * (g_j - sum_i g_i s_i / S) or scale * g_j;  dx = s (dS - sum s dS) or dS s (1 - s)
 //
-// One warp per token, expert e in register e / 32 of lane e % 32; a choice is topk rounds of a warp-wide maximum
-// over the lanes' best. Without a bias the scores are ordered as the logits are, and those are compared as they
-// stand. With one (or with sums of two scores over groups) the order is that of numbers fp32 may not tell apart:
-// each comparison that matters is checked against the bound of the fp32 scores' error, and a token that fails is
-// done again in fp64 (about 3 of 1000 at 256 experts).
+// One warp per token, expert e in register e / 32 of lane e % 32. The topk-th largest of the 32 lanes' maxima bounds
+// the topk-th value from below: what is not under it, some 10 to 20 candidates, is put one to a lane and ranked by
+// comparing each with each (16384 tokens, 256 experts, 8 chosen: kRouteNote). Where that leaves more than 32 (many
+// ties, a large topk), topk rounds of a warp-wide maximum choose. Without a bias the scores are ordered as the logits are, and those are compared as they
+// stand. With one (or with sums of two scores over groups) the order is that of numbers fp32 may not tell apart.
+// Every comparison that matters is checked against the bound of the fp32 scores' error; candidates closer than that
+// are put in order by their fp64 values (some 2 tokens of 1000 at 256 experts).
 #include <math.h>
 
 #include <type_traits>
@@ -22,6 +24,7 @@ namespace {
 
 constexpr int kRouteWarps = 4;
 constexpr uint32_t kAll = 0xFFFFFFFFu;
+constexpr int kMostRanked = 16;       // topk up to which the lanes' maxima leave few candidates
 
 __device__ __forceinline__ float load_logit(const void* p, int64_t i, bool bf16) {
   return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];
@@ -67,46 +70,79 @@ __device__ __forceinline__ void store_choice(const RouteArgs& a, int64_t token, 
   }
 }
 
-// One token with every score in fp64. `key` is the warp's shared memory, one word per expert.
-__device__ __noinline__ void route_exact(const RouteArgs& a, int64_t token, uint64_t* key) {
-  const int lane = threadIdx.x & 31, size = a.experts / a.groups;
-  double top = -INFINITY, sum = 0.0;
-  auto logit = [&](int e) { return static_cast<double>(load_logit(a.logits, token * a.ld_logits + e, a.bf16)); };
-  if (!a.sigmoid) {
+// A token's scores in fp64.
+struct ExactScores {
+  const RouteArgs& a;
+  int64_t token;
+  double top, sum;
+  __device__ __forceinline__ ExactScores(const RouteArgs& args, int64_t t) : a(args), token(t), top(0.0), sum(1.0) {
+    if (a.sigmoid) return;
+    const int lane = threadIdx.x & 31;
+    top = -INFINITY;
     for (int e = lane; e < a.experts; e += 32) top = fmax(top, logit(e));
     top = warp_max(top);
     if (top == -INFINITY) top = 0.0;
+    sum = 0.0;
     for (int e = lane; e < a.experts; e += 32) sum += exp(logit(e) - top);
     sum = warp_sum(sum);
   }
-  auto score = [&](double x) { return a.sigmoid ? 1.0 / (1.0 + exp(-x)) : sum == 0.0 ? 0.0 : exp(x - top) / sum; };
-  double* choice = reinterpret_cast<double*>(key);
-  __syncwarp();
-  for (int e = lane; e < a.experts; e += 32) {
+  __device__ __forceinline__ double logit(int e) const { return static_cast<double>(load_logit(a.logits, token * a.ld_logits + e, a.bf16)); }
+  __device__ __forceinline__ double score(double x) const { return a.sigmoid ? 1.0 / (1.0 + exp(-x)) : sum == 0.0 ? 0.0 : exp(x - top) / sum; }
+  __device__ __forceinline__ double choice(int e) const {
     const double x = logit(e);
-    choice[e] = x == -INFINITY ? x : a.bias != nullptr ? score(x) + static_cast<double>(a.bias[e]) : score(x);
+    return x == -INFINITY ? x : a.bias != nullptr ? score(x) + static_cast<double>(a.bias[e]) : score(x);
   }
+};
+
+// The groups a token keeps, from fp64 scores. `choice`: the warp's shared memory, a word per expert.
+__device__ __noinline__ uint32_t exact_groups(const RouteArgs& a, int64_t token, double* choice) {
+  const int lane = threadIdx.x & 31, size = a.experts / a.groups;
+  const ExactScores s(a, token);
   __syncwarp();
-  uint32_t kept = kAll;
-  if (a.groups > 1) {
-    double first = -INFINITY, second = -INFINITY;
-    if (lane < a.groups)
-      for (int e = lane * size; e < (lane + 1) * size; ++e) {
-        const double c = choice[e];
-        if (c > first) { second = first; first = c; }
-        else if (c > second) second = c;
-      }
-    const uint64_t mine = order_key(a.group_top2 && second > -INFINITY ? first + second : first);
-    int better = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      const uint64_t other = __shfl_sync(kAll, mine, g);
-      better += other > mine || (other == mine && g < lane);
+  for (int e = lane; e < a.experts; e += 32) choice[e] = s.choice(e);
+  __syncwarp();
+  double first = -INFINITY, second = -INFINITY;
+  if (lane < a.groups)
+    for (int e = lane * size; e < (lane + 1) * size; ++e) {
+      const double c = choice[e];
+      if (c > first) { second = first; first = c; }
+      else if (c > second) second = c;
     }
-    kept = __ballot_sync(kAll, lane < a.groups && better < a.topk_groups);
+  const uint64_t mine = order_key(a.group_top2 && second > -INFINITY ? first + second : first);
+  int better = 0;
+  for (int g = 0; g < a.groups; ++g) {
+    const uint64_t other = __shfl_sync(kAll, mine, g);
+    better += other > mine || (other == mine && g < lane);
   }
   __syncwarp();
-  for (int e = lane; e < a.experts; e += 32)
-    key[e] = !((kept >> (a.groups > 1 ? e / size : 0)) & 1u) ? 0 : order_key(a.bias != nullptr ? choice[e] : logit(e));
+  return __ballot_sync(kAll, lane < a.groups && better < a.topk_groups);
+}
+
+// Lanes 0 .. count - 1 hold candidates, among them all that may be chosen: in their order by fp64 choice values.
+__device__ __noinline__ int exact_order(const RouteArgs& a, int64_t token, int pick, int count) {
+  const int lane = threadIdx.x & 31;
+  const ExactScores s(a, token);
+  const uint64_t mine = lane < count ? order_key(s.choice(pick)) : 0;
+  int rank = 0;
+  for (int i = 0; i < count; ++i) {
+    const uint64_t other = __shfl_sync(kAll, mine, i);
+    const int e = __shfl_sync(kAll, pick, i);
+    rank += other > mine || (other == mine && e < pick);
+  }
+  int at = 0;
+  for (int i = 0; i < count; ++i) {
+    const int r = __shfl_sync(kAll, rank, i), e = __shfl_sync(kAll, pick, i);
+    if (r == lane) at = e;
+  }
+  return at;
+}
+
+// The whole choice in fp64, for more close candidates than a warp has lanes.
+__device__ __noinline__ int exact_choice(const RouteArgs& a, int64_t token, uint32_t kept, uint64_t* key) {
+  const int lane = threadIdx.x & 31, size = a.experts / a.groups;
+  const ExactScores s(a, token);
+  __syncwarp();
+  for (int e = lane; e < a.experts; e += 32) key[e] = !((kept >> (a.groups > 1 ? e / size : 0)) & 1u) ? 0 : order_key(s.choice(e));
   __syncwarp();
   int pick = 0;
   for (int j = 0; j < a.topk; ++j) {
@@ -124,7 +160,7 @@ __device__ __noinline__ void route_exact(const RouteArgs& a, int64_t token, uint
     if (lane == j) pick = at;
     __syncwarp();
   }
-  store_choice(a, token, lane, pick, lane < a.topk ? static_cast<float>(score(logit(pick))) : 0.0f);
+  return pick;
 }
 
 template <int NV>
@@ -134,151 +170,208 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t token = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
   if (token >= a.tokens) return;
-  uint64_t* scratch = shared + warp * a.experts;
-  float s[NV];
+  uint64_t* scratch = shared + warp * (a.experts + 32);
+  float c[NV];           // logits, then what a choice goes by
   uint32_t key[NV];
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int e = lane + 32 * i;
-    s[i] = e < a.experts ? load_logit(a.logits, token * a.ld_logits + e, a.bf16) : -INFINITY;
-    key[i] = e < a.experts ? order_key(s[i]) : 0;                 // the logits' order, for now
-    top = fmaxf(top, s[i]);
+    c[i] = e < a.experts ? load_logit(a.logits, token * a.ld_logits + e, a.bf16) : -INFINITY;
+    key[i] = e < a.experts ? order_key(c[i]) : 0;
+    top = fmaxf(top, c[i]);
   }
   const bool by_score = a.bias != nullptr;                        // else by logits
   const bool by_sum = a.groups > 1 && a.group_top2;
   float inv_sum = 1.0f;
-  if (a.sigmoid) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) s[i] = __fdividef(1.0f, 1.0f + expf(-s[i]));       // expf is at most 3e38 above: 1 / inf = 0
-  } else {
+  if (!a.sigmoid) {
     top = warp_max(top);
     if (top == -INFINITY) top = 0.0f;
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      s[i] = expf(s[i] - top);
-      sum += s[i];
-    }
+    for (int i = 0; i < NV; ++i) sum += expf(c[i] - top);
     sum = warp_sum(sum);
     inv_sum = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) s[i] *= inv_sum;
   }
-  // How far two fp32 choice values must lie apart to be in the order of the exact ones: twice the error of a score
-  // (expf 2 steps of 2^-23, sums and quotients at most NV + 8 half steps, |x - top| half steps where the score is
-  // exp(top - x) times smaller: together under (NV + 16) * 2^-23 of the largest score), and the rounding of the sums.
-  const float slack = (NV + 16) * 2.4e-7f * inv_sum;
-  auto near = [&](float high, float low) { return high - low <= slack + 4.8e-7f * (fabsf(high) + 0.25f); };   // NaN and inf - inf: not near
-  bool exact = true;
+  auto score = [&](float x) { return a.sigmoid ? 1.0f / (1.0f + expf(-x)) : expf(x - top) * inv_sum; };
+  // How far two fp32 choice values must lie apart to be in the order of the exact ones: twice the error of a score,
+  // and the roundings of the sums (under 2^-23 of |c| + 1/4 each). A sigmoid is off by the step of expf (2^-23), the
+  // sum's and the quotient's half steps: 2^-22 at most. A softmax by two steps of expf, the sum's NV + 5 roundings, two
+  // more, and half a step of |x - top|, which is largest against exp(top - x) at 1: under (NV + 12) 2^-23 of the largest.
+  const float slack = a.sigmoid ? 4.8e-7f : (NV + 12) * 2.4e-7f * inv_sum;
+  auto near = [&](float high, float low) { return high - low <= slack + 2.4e-7f * (fabsf(high) + 0.25f); };   // NaN and inf - inf: not near
   if (by_score || by_sum) {
-    float c[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int e = lane + 32 * i;
-      c[i] = e < a.experts ? (key[i] == 0x007FFFFFu ? -INFINITY : by_score ? s[i] + a.bias[e] : s[i]) : -INFINITY;
-      if (by_score && e < a.experts) key[i] = order_key(c[i]);
+      if (e >= a.experts) continue;
+      const float s = score(c[i]);
+      c[i] = c[i] == -INFINITY ? c[i] : by_score ? s + a.bias[e] : s;
+      if (by_score) key[i] = order_key(c[i]);
     }
-    if (a.groups > 1) {
-      float* choice = reinterpret_cast<float*>(scratch);
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (lane + 32 * i < a.experts) choice[lane + 32 * i] = c[i];
-    }
-  } else if (a.groups > 1) {
-    float* choice = reinterpret_cast<float*>(scratch);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (lane + 32 * i < a.experts) choice[lane + 32 * i] = key[i] == 1u ? NAN : key_value(key[i]);
   }
+  uint32_t kept = kAll;
   if (a.groups > 1) {
+    // `share` adjacent lanes look through a group; in shared memory each group starts `share` words on, so that the
+    // groups' lanes meet different banks
     const int size = a.experts / a.groups;
     const float inv_size = 1.0f / static_cast<float>(size);
-    const float* choice = reinterpret_cast<const float*>(scratch);
-    __syncwarp();
-    float first = -INFINITY, second = -INFINITY;
-    if (lane < a.groups)
-      for (int e = lane * size; e < (lane + 1) * size; ++e) {
-        const float c = choice[e];
-        second = fmaxf(second, fminf(first, c));     // fminf, fmaxf pass NaN over
-        first = fmaxf(first, c);
-      }
-    const float value = by_sum && second > -INFINITY ? first + second : first;
-    const uint32_t mine = order_key(value);
-    int better = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      const uint32_t other = __shfl_sync(kAll, mine, g);
-      better += other > mine || (other == mine && g < lane);
-    }
-    const bool keep = lane < a.groups && better < a.topk_groups;
-    const uint32_t kept = __ballot_sync(kAll, keep);
-    if (by_score || by_sum) {
-      const uint32_t worst_kept = __reduce_min_sync(kAll, keep ? mine : 0xFFFFFFFFu);
-      const uint32_t best_dropped = __reduce_max_sync(kAll, lane < a.groups && !keep ? mine : 0u);
-      exact = !near(key_value(worst_kept) * 0.5f, key_value(best_dropped) * 0.5f);       // sums of two have twice the error
-    }
+    auto group_of = [&](int e) { return static_cast<int>((static_cast<float>(e) + 0.5f) * inv_size); };   // exact up to 1024
+    int share = 32;
+    while (share * a.groups > 32) share >>= 1;
+    float* choice = reinterpret_cast<float*>(scratch);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int e = lane + 32 * i;
-      const int g = static_cast<int>((static_cast<float>(e) + 0.5f) * inv_size);
-      if (e < a.experts && !((kept >> g) & 1u)) key[i] = 0;
+      if (e < a.experts) choice[e + group_of(e) * share] = c[i];
     }
+    __syncwarp();
+    const int g = lane / share, sub = lane - g * share;
+    float first = -INFINITY, second = -INFINITY;
+    if (g < a.groups)
+      for (int e = sub; e < size; e += share) {
+        const float v = choice[g * (size + share) + e];
+        second = fmaxf(second, fminf(first, v));     // fminf, fmaxf pass NaN over
+        first = fmaxf(first, v);
+      }
+    for (int o = 1; o < share; o <<= 1) {
+      const float f = __shfl_xor_sync(kAll, first, o), h = __shfl_xor_sync(kAll, second, o);
+      second = fmaxf(fmaxf(second, h), fminf(first, f));
+      first = fmaxf(first, f);
+    }
+    const uint32_t mine = order_key(by_sum && second > -INFINITY ? first + second : first);
+    int better = 0;
+    for (int h = 0; h < a.groups; ++h) {
+      const uint32_t other = __shfl_sync(kAll, mine, h * share);
+      better += other > mine || (other == mine && h < g);
+    }
+    const bool keep = g < a.groups && better < a.topk_groups;
+    kept = 0;
+    const uint32_t lanes = __ballot_sync(kAll, keep);
+    for (int h = 0; h < a.groups; ++h) kept |= ((lanes >> (h * share)) & 1u) << h;
+    if (by_score || by_sum) {
+      const uint32_t worst_kept = __reduce_min_sync(kAll, keep ? mine : 0xFFFFFFFFu);
+      const uint32_t best_dropped = __reduce_max_sync(kAll, g < a.groups && !keep ? mine : 0u);
+      // sums of two have twice the error
+      if (near(key_value(worst_kept) * 0.5f, key_value(best_dropped) * 0.5f)) kept = exact_groups(a, token, reinterpret_cast<double*>(scratch));
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (lane + 32 * i < a.experts && !((kept >> group_of(lane + 32 * i)) & 1u)) key[i] = 0;
   }
-  int pick = 0;          // lane j: the j-th chosen expert
   uint32_t best = 0;     // this lane's best candidate and its register
   int slot = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (key[i] > best) { best = key[i]; slot = i; }
-  uint32_t last = 0;     // the key chosen before, and its expert
-  int last_at = 0;
-  const int rounds = by_score ? a.topk + 1 : a.topk;               // one more value is looked at than chosen
-  for (int j = 0; j < rounds; ++j) {
-    const uint32_t m = __reduce_max_sync(kAll, best);
-    const int at = __reduce_min_sync(kAll, best == m ? lane + 32 * slot : 0x7FFFFFFF);
-    // near values are in order only if they are the same number: the same logit under the same bias
-    if (by_score && j > 0 && m > 1u && near(key_value(last), key_value(m)))
-      exact = exact && a.bias[at] == a.bias[last_at] &&
-              load_logit(a.logits, token * a.ld_logits + at, a.bf16) == load_logit(a.logits, token * a.ld_logits + last_at, a.bf16);
-    last = m;
-    last_at = at;
-    if (j == a.topk) break;
-    if (lane == (at & 31)) {
-      best = 0;
+  int pick = 0;          // lane j: the j-th candidate, best first
+  int count = 33;
+  bool close = false;
+  if (a.topk <= kMostRanked) {
+    uint32_t bound = 0, v = best;
+    for (int j = 0; j < a.topk; ++j) {                               // equal maxima go together, which only lowers the bound
+      bound = __reduce_max_sync(kAll, v);
+      if (v == bound) v = 0;
+    }
+    // with scores: also what may change places with a chosen one
+    if (by_score && bound > 1u) {
+      const float x = key_value(bound);
+      const float low = x - (slack + 2.4e-7f * (fabsf(x) + 0.25f)) * 1.001f;
+      if (low == low) bound = order_key(low);
+    }
+    if (bound == 0) bound = 1;
+    uint32_t* list = reinterpret_cast<uint32_t*>(scratch);           // keys, then experts
+    int n = 0;
+    __syncwarp();
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        key[i] = at == lane + 32 * i ? 0 : key[i];
-        if (key[i] > best) { best = key[i]; slot = i; }
+    for (int i = 0; i < NV; ++i) {
+      const bool in = key[i] >= bound;
+      const uint32_t lanes = __ballot_sync(kAll, in);
+      const int at = n + __popc(lanes & ((1u << lane) - 1u));
+      if (in && at < 32) {
+        list[at] = key[i];
+        list[32 + at] = lane + 32 * i;
+      }
+      n += __popc(lanes);
+    }
+    __syncwarp();
+    if (n <= 32) {
+      // the list is in the order of the experts, so among equal keys the earlier place is the lower index
+      const uint32_t mine = lane < n ? list[lane] : 0;
+      const int e = lane < n ? list[32 + lane] : 0;
+      int rank = 0;
+      for (int j = 0; j < n; ++j) {
+        const uint32_t other = list[j];
+        rank += other > mine || (other == mine && j < lane);
+      }
+      __syncwarp();
+      if (lane < n) {
+        list[rank] = mine;
+        list[32 + rank] = e;
+      }
+      __syncwarp();
+      count = n;
+      pick = lane < n ? list[32 + lane] : 0;
+      if (by_score) {
+        // neighbours that near are in order only if they are the same number: the same logit under the same bias
+        const bool follows = lane > 0 && lane < n && lane <= a.topk && list[lane] > 1u && near(key_value(list[lane - 1]), key_value(list[lane]));
+        bool differ = false;
+        if (follows) {
+          const int before = list[32 + lane - 1];
+          differ = a.bias[pick] != a.bias[before] ||
+                   load_logit(a.logits, token * a.ld_logits + pick, a.bf16) != load_logit(a.logits, token * a.ld_logits + before, a.bf16);
+        }
+        close = __any_sync(kAll, differ);
       }
     }
-    if (lane == j) pick = at;
   }
-  if (!exact) {
-    route_exact(a, token, scratch);
-    return;
+  if (count > 32) {
+    uint32_t last = 0;     // the key chosen before, and its expert
+    int last_at = 0;
+    for (count = 0;; ++count) {
+      const uint32_t m = __reduce_max_sync(kAll, best);
+      // past topk as long as a candidate may still change places with a chosen one
+      const bool follows = by_score && count > 0 && m > 1u && near(key_value(last), key_value(m));
+      if (count >= a.topk && (!follows || count == 32)) {
+        if (follows) count = 33;
+        break;
+      }
+      const int at = __reduce_min_sync(kAll, best == m ? lane + 32 * slot : 0x7FFFFFFF);
+      if (follows)
+        close = close || a.bias[at] != a.bias[last_at] ||
+                load_logit(a.logits, token * a.ld_logits + at, a.bf16) != load_logit(a.logits, token * a.ld_logits + last_at, a.bf16);
+      last = m;
+      last_at = at;
+      if (lane == (at & 31)) {
+        best = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          key[i] = at == lane + 32 * i ? 0 : key[i];
+          if (key[i] > best) { best = key[i]; slot = i; }
+        }
+      }
+      if (lane == count) pick = at;
+    }
   }
-  float weight = 0.0f;
-  if (lane < a.topk) {
-    const float x = load_logit(a.logits, token * a.ld_logits + pick, a.bf16);
-    weight = a.sigmoid ? __fdividef(1.0f, 1.0f + expf(-x)) : expf(x - top) * inv_sum;
-  }
-  store_choice(a, token, lane, pick, weight);
+  if (count > 32) pick = exact_choice(a, token, kept, scratch);
+  else if (close) pick = exact_order(a, token, pick, count);
+  store_choice(a, token, lane, pick, lane < a.topk ? score(load_logit(a.logits, token * a.ld_logits + pick, a.bf16)) : 0.0f);
 }
 
 template <int NV>
 __global__ void __launch_bounds__(kRouteWarps * 32)
-route_topk_bwd_kernel(const RouteBwdArgs a) {
+route_topk_bwd_kernel(const __grid_constant__ RouteBwdArgs a) {
+  extern __shared__ float ds_all[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t token = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
   if (token >= a.tokens) return;
-  float s[NV], ds[NV];
+  float s[NV];
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int e = lane + 32 * i;
     s[i] = e < a.experts ? load_logit(a.logits, token * a.ld_logits + e, a.bf16) : -INFINITY;
     top = fmaxf(top, s[i]);
-    ds[i] = 0.0f;
   }
   top = warp_max(top);
   if (top == -INFINITY) top = 0.0f;
@@ -307,20 +400,26 @@ route_topk_bwd_kernel(const RouteBwdArgs a) {
     g = !valid || total == 0.0f ? 0.0f : (g - inner / total) / total;
   }
   const float dot = a.sigmoid ? 0.0f : warp_sum(g * mine);
-  for (int j = 0; j < a.topk; ++j) {
-    const int e = __shfl_sync(kAll, at, j);
-    const float v = __shfl_sync(kAll, g, j);
-    if ((e & 31) == lane) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (e == lane + 32 * i) ds[i] += v;
+  // slots to experts, in the slots' order (an expert may be named twice)
+  float* ds = ds_all + warp * a.experts;
+  for (int e = lane; e < a.experts; e += 32) ds[e] = 0.0f;
+  __syncwarp();
+  const uint32_t peers = __match_any_sync(kAll, valid ? at : -1 - lane);
+  const bool alone = __all_sync(kAll, peers == 1u << lane);
+  if (alone) {
+    if (valid) ds[at] = g;
+  } else {
+    for (int j = 0; j < a.topk; ++j) {
+      if (lane == j && valid) ds[at] += g;
+      __syncwarp();
     }
   }
+  __syncwarp();
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int e = lane + 32 * i;
     if (e >= a.experts) continue;
-    const float d = a.sigmoid ? ds[i] * s[i] * (1.0f - s[i]) : s[i] * (ds[i] - dot);
+    const float d = a.sigmoid ? ds[e] * s[i] * (1.0f - s[i]) : s[i] * (ds[e] - dot);
     const int64_t o = token * a.experts + e;
     if (a.bf16) static_cast<__nv_bfloat16*>(a.d_logits)[o] = __float2bfloat16_rn(d);
     else static_cast<float*>(a.d_logits)[o] = d;
@@ -345,14 +444,14 @@ cudaError_t launch_route_topk(const RouteArgs& a, cudaStream_t stream) {
   if (a.tokens == 0) return cudaSuccess;
   const unsigned grid = static_cast<unsigned>((a.tokens + kRouteWarps - 1) / kRouteWarps);
   return by_width(a.experts, [&](auto n) {
-    route_topk_kernel<decltype(n)::value><<<grid, kRouteWarps * 32, kRouteWarps * a.experts * sizeof(uint64_t), stream>>>(a);
+    route_topk_kernel<decltype(n)::value><<<grid, kRouteWarps * 32, kRouteWarps * (a.experts + 32) * sizeof(uint64_t), stream>>>(a);
   });
 }
 
 cudaError_t launch_route_topk_bwd(const RouteBwdArgs& a, cudaStream_t stream) {
   if (a.tokens == 0) return cudaSuccess;
   const unsigned grid = static_cast<unsigned>((a.tokens + kRouteWarps - 1) / kRouteWarps);
-  return by_width(a.experts, [&](auto n) { route_topk_bwd_kernel<decltype(n)::value><<<grid, kRouteWarps * 32, 0, stream>>>(a); });
+  return by_width(a.experts, [&](auto n) { route_topk_bwd_kernel<decltype(n)::value><<<grid, kRouteWarps * 32, kRouteWarps * a.experts * sizeof(float), stream>>>(a); });
 }
 
 }  // namespace plb

@@ -64,11 +64,11 @@ def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
         r2, ld_r = rows_of(residual) if residual is not None else (None, 0)
         weight = dense(weight)
         if into is None:
-            into = Normed(torch.empty(shape, dtype=torch.bfloat16, device=dev) if residual is not None else x,
-                          torch.empty(rows, dtype=torch.float32, device=dev),
-                          torch.empty(shape, dtype=torch.bfloat16, device=dev) if out != "mxfp8" else None,
-                          torch.empty((padded, width), dtype=torch.uint8, device=dev) if out != "bf16" else None,
-                          torch.empty((padded // 128, width // 128, 32, 16), dtype=torch.uint8, device=dev) if out != "bf16" else None)
+            into = Normed(x.new_empty(shape) if residual is not None else x,
+                          x.new_empty(rows, dtype=torch.float32),
+                          x.new_empty(shape) if out != "mxfp8" else None,
+                          x.new_empty((padded, width), dtype=torch.uint8) if out != "bf16" else None,
+                          x.new_empty((padded // 128, width // 128, 32, 16), dtype=torch.uint8) if out != "bf16" else None)
         else:
             _check_into(into, residual, out, rows, width, padded, dev)
         _lib.call("plb_rmsnorm_fwd", x2.data_ptr(), ld_x, _ptr(r2), ld_r, weight.data_ptr(), rows, width, eps,
@@ -99,10 +99,10 @@ def rmsnorm_bwd(d_y: torch.Tensor, hidden: torch.Tensor, rstd: torch.Tensor, wei
         h2, ld_h = rows_of(hidden)
         e2, ld_e = rows_of(d_hidden) if d_hidden is not None else (None, 0)
         rstd, weight = rstd.contiguous(), dense(weight)
-        d_x = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-        d_weight = torch.empty(width, dtype=torch.float32, device=dev)
+        d_x = hidden.new_empty(shape)
+        d_weight = hidden.new_empty(width, dtype=torch.float32)
         nbytes = _lib.load().plb_rmsnorm_bwd_workspace_bytes(rows, width)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        workspace = hidden.new_empty(nbytes, dtype=torch.uint8)
         _lib.call("plb_rmsnorm_bwd", g2.data_ptr(), ld_g, h2.data_ptr(), ld_h, rstd.data_ptr(), weight.data_ptr(), _ptr(e2), ld_e,
                   rows, width, d_x.data_ptr(), d_weight.data_ptr(), workspace.data_ptr(), nbytes, _stream())
     return d_x, d_weight

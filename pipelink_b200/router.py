@@ -50,8 +50,8 @@ def route_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias:
         x, ld = rows_of(logits)
         bias = bias.contiguous() if bias is not None else None
         if into is None:
-            chosen = torch.empty((tokens, topk), dtype=torch.int32, device=dev)
-            weights = torch.empty((tokens, topk), dtype=torch.float32, device=dev)
+            chosen = logits.new_empty((tokens, topk), dtype=torch.int32)
+            weights = logits.new_empty((tokens, topk), dtype=torch.float32)
         else:
             chosen, weights = into
             for t, dtype in ((chosen, torch.int32), (weights, torch.float32)):
@@ -79,7 +79,7 @@ def route_topk_bwd(d_weights: torch.Tensor, logits: torch.Tensor, experts: torch
     with device_of(logits):
         x, ld = rows_of(logits)
         d_weights, experts = d_weights.contiguous(), experts.contiguous()
-        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        d_logits = logits.new_empty(logits.shape)
         _lib.call("plb_route_topk_bwd", d_weights.data_ptr(), x.data_ptr(), ld, int(x.dtype == torch.bfloat16), experts.data_ptr(),
                   tokens, logits.shape[1], topk, _SCORES[score], int(renormalize), float(scale), d_logits.data_ptr(), _stream())
     return d_logits
