@@ -7,7 +7,7 @@
 // the statistics are fp32; y is rounded to bf16 before it is quantised, so the bytes are those of
 // plb_mxfp8_quantize on y.
 //
-// Both directions are bound by memory: a row is read once into registers, reduced by the TPR threads that hold it
+// Both directions are bound by memory: a row is read once into registers, reduced by the threads that hold it
 // and written from there. VEC is the elements a thread moves at a time: 8 (16 bytes) where width, strides and
 // addresses allow, else 1. Rows too wide for registers (16384 elements, 8192 unaligned) are read twice.
 #include <type_traits>
@@ -50,8 +50,8 @@ struct Chunk;
 template <>
 struct Chunk<8> {
   uint4 raw;
-  __device__ __forceinline__ void load(const void* base, int64_t i) { raw = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + i); }
-  __device__ __forceinline__ void store(void* base, int64_t i) const { *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(base) + i) = raw; }
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { raw = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void store(__nv_bfloat16* p) const { *reinterpret_cast<uint4*>(p) = raw; }
   __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ float get(int i) const {
     const uint32_t w = i < 2 ? raw.x : i < 4 ? raw.y : i < 6 ? raw.z : raw.w;
@@ -64,69 +64,78 @@ struct Chunk<8> {
 template <>
 struct Chunk<1> {
   __nv_bfloat16 raw;
-  __device__ __forceinline__ void load(const void* base, int64_t i) { raw = static_cast<const __nv_bfloat16*>(base)[i]; }
-  __device__ __forceinline__ void store(void* base, int64_t i) const { static_cast<__nv_bfloat16*>(base)[i] = raw; }
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { raw = *p; }
+  __device__ __forceinline__ void store(__nv_bfloat16* p) const { *p = raw; }
   __device__ __forceinline__ void zero() { raw = __float2bfloat16_rn(0.0f); }
   __device__ __forceinline__ float get(int) const { return __bfloat162float(raw); }
   __device__ __forceinline__ void set(const float (&f)[1]) { raw = __float2bfloat16_rn(f[0]); }
 };
 
-// CTAs hold whole rows: several where a warp has a row to itself, one otherwise.
-template <int TPR>
+// The SIZE threads of a row: a warp (eight rows a CTA, no barriers) or a whole CTA. A compile-time size: with the
+// exact number of warps a width needs, known at run time only, 16384 x 4096 takes 94 us instead of 91.
+template <int SIZE>
 struct RowTeam {
-  static constexpr int kThreads = TPR < kNormThreads ? kNormThreads : TPR;
-  static constexpr int kRows = kThreads / TPR;
+  static constexpr int kThreads = SIZE == 32 ? kNormThreads : SIZE, kRows = kThreads / SIZE;
+  __device__ static __forceinline__ int thread() { return threadIdx.x % SIZE; }
+  __device__ static __forceinline__ int row() { return threadIdx.x / SIZE; }
   // Sum over a row's threads, the same bits in each; `round` alternates the buffers of consecutive sums.
   __device__ static __forceinline__ float sum(float v, int round) {
     v = warp_sum(v);
-    if constexpr (TPR > 32) {
-      __shared__ float part[2][kThreads / 32];
-      if ((threadIdx.x & 31) == 0) part[round & 1][threadIdx.x >> 5] = v;
+    if constexpr (SIZE > 32) {
+      __shared__ float part[2][32];
+      const int lane = threadIdx.x & 31;
+      if (lane == 0) part[round & 1][threadIdx.x >> 5] = v;
       __syncthreads();
-      v = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) v += part[round & 1][i];
+      v = warp_sum(lane < SIZE / 32 ? part[round & 1][lane] : 0.0f);
     }
     return v;
   }
 };
 
-template <int VEC, int TPR, int NV>
-__global__ void __launch_bounds__(RowTeam<TPR>::kThreads)
-rmsnorm_fwd_rows(const NormFwdArgs a) {
-  using Team = RowTeam<TPR>;
-  const int t = threadIdx.x % TPR;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * Team::kRows + threadIdx.x / TPR;
+// NV chunks of VEC elements a thread. Threads per SM by what a thread holds, the registers it needs without spilling:
+// 2048 for 8 elements (16384 x 2048: 44 us with one register more, 41 so), 1280 for 16 (16384 x 4096 with both outputs:
+// 100 us with 1024, 91 so), 1024 for 32.
+template <int VEC, int SIZE, int NV>
+__global__ void __launch_bounds__(RowTeam<SIZE>::kThreads, (NV * VEC <= 8 ? 2048 : NV * VEC <= 16 ? 1280 : 1024) / RowTeam<SIZE>::kThreads)
+rmsnorm_fwd_rows(const __grid_constant__ NormFwdArgs a) {
+  using Team = RowTeam<SIZE>;
+  const int t = Team::thread();
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * Team::kRows + Team::row();
   const bool live = row < a.rows;
-  const int64_t width = a.width;
+  const int width = static_cast<int>(a.width);
+  const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(a.x) + row * a.ld_x;
+  const __nv_bfloat16* residual = static_cast<const __nv_bfloat16*>(a.residual) + row * a.ld_residual;
+  const __nv_bfloat16* weight = static_cast<const __nv_bfloat16*>(a.weight);
+  __nv_bfloat16* hidden = static_cast<__nv_bfloat16*>(a.hidden) + row * width;
+  __nv_bfloat16* y_out = static_cast<__nv_bfloat16*>(a.y) + row * width;
   Chunk<VEC> h[NV], w[NV];
   float sq = 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+    const int c = (t + i * SIZE) * VEC;
     h[i].zero();
     w[i].zero();
     if (c < width) {
-      if (live) h[i].load(a.x, row * a.ld_x + c);
-      w[i].load(a.weight, c);
+      if (live) h[i].load(x + c);
+      w[i].load(weight + c);
     }
   }
   if (a.residual != nullptr && live) {
     Chunk<VEC> r[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
-      if (c < width) r[i].load(a.residual, row * a.ld_residual + c);
+      const int c = (t + i * SIZE) * VEC;
+      if (c < width) r[i].load(residual + c);
       else r[i].zero();
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+      const int c = (t + i * SIZE) * VEC;
       float f[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) f[e] = h[i].get(e) + r[i].get(e);
       h[i].set(f);
-      if (c < width) h[i].store(a.hidden, row * width + c);
+      if (c < width) h[i].store(hidden + c);
     }
   }
 #pragma unroll
@@ -139,15 +148,15 @@ rmsnorm_fwd_rows(const NormFwdArgs a) {
   if (!live && !(quantise && row < (a.rows + 127) / 128 * 128)) return;     // MXFP8 rows up to a multiple of 128 are zeros
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+    const int c = (t + i * SIZE) * VEC;
     const bool in = c < width;
-    if (i * TPR * VEC >= width) break;            // the same for every thread of the row
+    if (i * SIZE * VEC >= width) break;            // the same for every thread of the row
     float f[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) f[e] = h[i].get(e) * rstd * w[i].get(e);
     Chunk<VEC> y;
     y.set(f);
-    if (live && in && a.y != nullptr) y.store(a.y, row * width + c);
+    if (live && in && a.y != nullptr) y.store(y_out + c);
     if (!quantise) continue;
     // 32 / VEC adjacent lanes hold a block; width is a multiple of 128, so a block is wholly inside the row or outside
     float amax = 0.0f;
@@ -183,12 +192,18 @@ rmsnorm_fwd_rows(const NormFwdArgs a) {
 
 // The gradient of x, and this CTA's share of the weight's: a thread keeps the sums of its columns over the rows
 // the CTA walks, so dy and h are read once for both.
-template <int VEC, int TPR, int NV>
-__global__ void __launch_bounds__(RowTeam<TPR>::kThreads)
-rmsnorm_bwd_rows(const NormBwdArgs a) {
-  using Team = RowTeam<TPR>;
-  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
-  const int64_t width = a.width, sets = (a.rows + Team::kRows - 1) / Team::kRows;
+//
+// CTAs per SM: 1024 threads where a thread holds 8 elements, 512 (128 registers) where it holds more or loads ahead; 768
+// threads of 16 elements spill (16384 x 4096: 114 us, with 512 threads 104).
+template <int VEC, int SIZE, int NV>
+constexpr int kBwdResident = SIZE == 1024 ? 1 : (SIZE == 32 || NV * VEC > 8 ? 512 : 1024) / RowTeam<SIZE>::kThreads;
+template <int VEC, int SIZE, int NV>
+__global__ void __launch_bounds__(RowTeam<SIZE>::kThreads, kBwdResident<VEC, SIZE, NV>)
+rmsnorm_bwd_rows(const __grid_constant__ NormBwdArgs a) {
+  using Team = RowTeam<SIZE>;
+  const int t = Team::thread(), team = Team::row();
+  const int width = static_cast<int>(a.width);
+  const int64_t sets = (a.rows + Team::kRows - 1) / Team::kRows;
   const float inv_width = 1.0f / static_cast<float>(width);
   float dw[NV][VEC];
 #pragma unroll
@@ -200,38 +215,61 @@ rmsnorm_bwd_rows(const NormBwdArgs a) {
   Chunk<VEC> kept[kKeepWeight ? NV : 1];
   auto weight = [&](int i) {
     if constexpr (kKeepWeight) return kept[i];
-    const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+    const int c = (t + i * SIZE) * VEC;
     Chunk<VEC> v;
     v.zero();
-    if (c < width) v.load(a.weight, c);
+    if (c < width) v.load(static_cast<const __nv_bfloat16*>(a.weight) + c);
     return v;
   };
   if constexpr (kKeepWeight) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+      const int c = (t + i * SIZE) * VEC;
       kept[i].zero();
-      if (c < width) kept[i].load(a.weight, c);
+      if (c < width) kept[i].load(static_cast<const __nv_bfloat16*>(a.weight) + c);
     }
   }
+  struct Row { Chunk<VEC> g[NV], h[NV], r[NV]; float rstd; };
+  auto fetch = [&](Row& v, int64_t set) {
+    const int64_t row = set * Team::kRows + team;
+    const bool live = row < a.rows;
+    const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(a.d_y) + row * a.ld_d_y;
+    const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(a.hidden) + row * a.ld_hidden;
+    const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(a.d_hidden) + row * a.ld_d_hidden;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (t + i * SIZE) * VEC;
+      v.g[i].zero();
+      v.h[i].zero();
+      v.r[i].zero();
+      if (live && c < width) {
+        v.g[i].load(g + c);
+        v.h[i].load(h + c);
+        if (a.d_hidden != nullptr) v.r[i].load(r + c);
+      }
+    }
+    v.rstd = live ? a.rstd[row] : 0.0f;
+  };
+  // a warp that has a row to itself loads the next while it sums this one (65536 x 512: 48 us without, 46 with); CTAs
+  // of several warps do not gain from it
+  constexpr bool kAhead = SIZE == 32 && NV * VEC <= 16;
+  Row next;
+  if (kAhead) fetch(next, blockIdx.x);
   int round = 0;
   for (int64_t set = blockIdx.x; set < sets; set += gridDim.x, ++round) {
     const int64_t row = set * Team::kRows + team;
     const bool live = row < a.rows;
-    Chunk<VEC> g[NV], h[NV], r[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
-      g[i].zero();
-      h[i].zero();
-      r[i].zero();
-      if (live && c < width) {
-        g[i].load(a.d_y, row * a.ld_d_y + c);
-        h[i].load(a.hidden, row * a.ld_hidden + c);
-        if (a.d_hidden != nullptr) r[i].load(a.d_hidden, row * a.ld_d_hidden + c);
-      }
+    Row now;
+    if (kAhead) {
+      now = next;
+      if (set + gridDim.x < sets) fetch(next, set + gridDim.x);
+    } else {
+      fetch(now, set);
     }
-    const float rstd = live ? a.rstd[row] : 0.0f;
+    Chunk<VEC>(&g)[NV] = now.g;
+    Chunk<VEC>(&h)[NV] = now.h;
+    Chunk<VEC>(&r)[NV] = now.r;
+    const float rstd = now.rstd;
     float dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -245,9 +283,10 @@ rmsnorm_bwd_rows(const NormBwdArgs a) {
     }
     const float mean = Team::sum(dot, round) * inv_width;
     if (!live) continue;
+    __nv_bfloat16* d_x = static_cast<__nv_bfloat16*>(a.d_x) + row * width;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+      const int c = (t + i * SIZE) * VEC;
       if (c >= width) continue;
       const Chunk<VEC> w = weight(i);
       float d[VEC];
@@ -256,11 +295,11 @@ rmsnorm_bwd_rows(const NormBwdArgs a) {
         d[e] = fmaf(rstd, fmaf(-h[i].get(e) * rstd, mean, g[i].get(e) * w.get(e)), r[i].get(e));
       Chunk<VEC> out;
       out.set(d);
-      out.store(a.d_x, row * width + c);
+      out.store(d_x + c);
     }
   }
   if constexpr (Team::kRows > 1) {                 // the CTA's rows of each column, in their order
-    __shared__ float part[Team::kThreads][NV * VEC];
+    __shared__ float part[kNormThreads][NV * VEC];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -271,14 +310,14 @@ rmsnorm_bwd_rows(const NormBwdArgs a) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
-        for (int k = 1; k < Team::kRows; ++k) dw[i][e] += part[k * TPR + t][i * VEC + e];
+        for (int k = 1; k < Team::kRows; ++k) dw[i][e] += part[k * 32 + t][i * VEC + e];
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int64_t c = (t + static_cast<int64_t>(i) * TPR) * VEC;
+    const int c = (t + i * SIZE) * VEC;
     if (c >= width) continue;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) a.workspace[blockIdx.x * width + c + e] = dw[i][e];
+    for (int e = 0; e < VEC; ++e) a.workspace[static_cast<int64_t>(blockIdx.x) * width + c + e] = dw[i][e];
   }
 }
 
@@ -352,32 +391,35 @@ rmsnorm_dw_wide(const NormBwdArgs a, int64_t rows_per_strip) {
   a.workspace[blockIdx.y * a.width + c] = s;
 }
 
-// d_weight = sum over the strips: 32 columns a CTA, 8 strips at a time, the eight partial sums joined in their order.
-__global__ void __launch_bounds__(kNormThreads)
+// d_weight = sum over the strips: 32 columns a CTA, a strip a warp, the warps' sums joined in their order. 32 warps
+// so that a few loads in flight per thread cover all strips (444 strips of 4096: kSumNote).
+constexpr int kSumThreads = 1024;
+__global__ void __launch_bounds__(kSumThreads)
 rmsnorm_dw_sum(const float* __restrict__ partial, int strips, int64_t width, float* __restrict__ d_weight) {
-  __shared__ float part[kNormThreads / 32][32];
+  __shared__ float part[kSumThreads / 32][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float s = 0.0f;
   if (c < width)
-#pragma unroll 4
-    for (int i = warp; i < strips; i += kNormThreads / 32) s += partial[i * width + c];
+#pragma unroll 8
+    for (int i = warp; i < strips; i += kSumThreads / 32) s += partial[i * width + c];
   part[warp][lane] = s;
   __syncthreads();
   if (warp != 0 || c >= width) return;
 #pragma unroll
-  for (int i = 1; i < kNormThreads / 32; ++i) s += part[i][lane];
+  for (int i = 1; i < kSumThreads / 32; ++i) s += part[i][lane];
   d_weight[c] = s;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <int V, int T, int N>
+template <int V, int S, int N>
 struct RowShape {
-  static constexpr int kVec = V, kTpr = T, kNv = N;
+  static constexpr int kVec = V, kSize = S, kNv = N;
 };
 // Calls f with the row shape for a width, false where rows do not fit in registers. Rows that a warp can hold get a
-// warp, which needs no barrier; few wide rows get the largest team, as the time of one row is what counts then.
+// warp, wider ones a CTA of 256 threads as long as those can hold them, and few rows as many threads as they fill,
+// since the time of one row is what counts there (1 x 4096: 2.4 us with 512 threads).
 template <class F>
 bool by_row_shape(bool vec, int64_t width, bool few, F&& f) {
   if (vec) {
@@ -387,15 +429,16 @@ bool by_row_shape(bool vec, int64_t width, bool few, F&& f) {
     else if (n <= 128) f(RowShape<8, 32, 4>{});
     else if (n <= 256) f(RowShape<8, 256, 1>{});
     else if (few && n <= 512) f(RowShape<8, 512, 1>{});
+    else if (few && n <= 1024) f(RowShape<8, 1024, 1>{});
     else if (n <= 512) f(RowShape<8, 256, 2>{});
-    else if (n <= 1024) f(RowShape<8, 512, 2>{});
+    else if (n <= 1024) f(RowShape<8, 256, 4>{});
     else if (n <= 2048) f(RowShape<8, 512, 4>{});
     else return false;
   } else {
     if (width <= 128) f(RowShape<1, 32, 4>{});
     else if (width <= 1024) f(RowShape<1, 256, 4>{});
     else if (width <= 4096) f(RowShape<1, 256, 16>{});
-    else if (width <= 8192) f(RowShape<1, 512, 16>{});
+    else if (width <= 8192) f(RowShape<1, 1024, 8>{});
     else return false;
   }
   return true;
@@ -412,8 +455,8 @@ cudaError_t launch_rmsnorm_fwd(const NormFwdArgs& a, cudaStream_t stream) {
                    aligned16(a.weight) && aligned16(a.hidden) && aligned16(a.y);
   const bool done = by_row_shape(vec, a.width, a.rows <= a.num_sms, [&](auto s) {
     using S = decltype(s);
-    using Team = RowTeam<S::kTpr>;
-    rmsnorm_fwd_rows<S::kVec, S::kTpr, S::kNv><<<static_cast<unsigned>((rows + Team::kRows - 1) / Team::kRows), Team::kThreads, 0, stream>>>(a);
+    using Team = RowTeam<S::kSize>;
+    rmsnorm_fwd_rows<S::kVec, S::kSize, S::kNv><<<static_cast<unsigned>((rows + Team::kRows - 1) / Team::kRows), Team::kThreads, 0, stream>>>(a);
   });
   if (!done) rmsnorm_fwd_wide<<<static_cast<unsigned>(rows), kNormThreads, 0, stream>>>(a);
   return cudaGetLastError();
@@ -425,13 +468,13 @@ cudaError_t launch_rmsnorm_bwd(const NormBwdArgs& a, cudaStream_t stream) {
   int64_t strips = norm_bwd_strips(a.rows);
   const bool done = by_row_shape(vec, a.width, a.rows <= a.num_sms, [&](auto s) {
     using S = decltype(s);
-    using Team = RowTeam<S::kTpr>;
+    using Team = RowTeam<S::kSize>;
     const int64_t sets = (a.rows + Team::kRows - 1) / Team::kRows;
-    const int64_t most = static_cast<int64_t>(a.num_sms) * (Team::kThreads > 256 ? 1 : 3);
+    const int64_t most = static_cast<int64_t>(a.num_sms) * kBwdResident<S::kVec, S::kSize, S::kNv>;
     strips = sets < 1 ? 1 : sets;
     if (strips > most) strips = most;
     if (strips > kNormMaxStrips) strips = kNormMaxStrips;
-    rmsnorm_bwd_rows<S::kVec, S::kTpr, S::kNv><<<static_cast<unsigned>(strips), Team::kThreads, 0, stream>>>(a);
+    rmsnorm_bwd_rows<S::kVec, S::kSize, S::kNv><<<static_cast<unsigned>(strips), Team::kThreads, 0, stream>>>(a);
   });
   if (!done) {
     const int64_t per = (a.rows + strips - 1) / strips;
@@ -443,7 +486,7 @@ cudaError_t launch_rmsnorm_bwd(const NormBwdArgs& a, cudaStream_t stream) {
   }
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
-  rmsnorm_dw_sum<<<static_cast<unsigned>((a.width + 31) / 32), kNormThreads, 0, stream>>>(a.workspace, static_cast<int>(strips), a.width, a.d_weight);
+  rmsnorm_dw_sum<<<static_cast<unsigned>((a.width + 31) / 32), kSumThreads, 0, stream>>>(a.workspace, static_cast<int>(strips), a.width, a.d_weight);
   return cudaGetLastError();
 }
 
