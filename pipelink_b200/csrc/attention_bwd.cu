@@ -145,9 +145,23 @@ struct KvWalk {
   }
 };
 
-// A role's wait: the warp's lanes agree on the outcome.
+// A role's bounded wait; the warp's lanes agree on the outcome. Without a status record a wait that runs out goes
+// unreported, and the CTA's others run out by themselves.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, Status* st, int code, int what) {
-  return __all_sync(kFullMask, mbar_wait(bar, parity, st, code, what)) != 0;
+  bool ok = true;
+  if (!mbar_try_wait(bar, parity)) {
+    const long long t0 = clock64();
+    for (uint32_t it = 1; !mbar_try_wait(bar, parity); ++it) {
+      if ((it & 63u) != 0u) continue;
+      if (st != nullptr && ld_volatile_i32(&st->code) != 0) { ok = false; break; }
+      if (clock64() - t0 > kWaitBudgetCycles) {
+        if (st != nullptr) report_failure(st, code, what, parity, bar);
+        ok = false;
+        break;
+      }
+    }
+  }
+  return __all_sync(kFullMask, ok) != 0;
 }
 // A compute warp's arrival: one for its 32 lanes (32 arrivals on one barrier are 32 shared-memory atomics in a row,
 // and with two barriers a tile those took a quarter of the compute warps' time).
@@ -224,30 +238,6 @@ __device__ __forceinline__ void linger() {   // copies in flight land before the
   }
 }
 
-// Two fp32 lanes of one register pair: Blackwell's packed arithmetic takes one issue slot for both.
-struct Pair { uint64_t v; };
-__device__ __forceinline__ Pair make_pair(float a, float b) {
-  Pair r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ Pair make_pair(uint32_t a, uint32_t b) { return make_pair(__uint_as_float(a), __uint_as_float(b)); }
-__device__ __forceinline__ void split(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
 __device__ __forceinline__ Pair exp2_pair(Pair x) {
   float a, b;
   split(x, a, b);
@@ -347,7 +337,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sb = smem_u32(smem);
   if ((sb & 1023u) != 0) {          // the swizzle pattern repeats every 1024 bytes
-    if (threadIdx.x == 0) report_failure(p.status, ST_BAD_ARGUMENT, 499, sb, 1024);
+    if (threadIdx.x == 0 && p.status != nullptr) report_failure(p.status, ST_BAD_ARGUMENT, 499, sb, 1024);
     return;
   }
   DqBars* bars = reinterpret_cast<DqBars*>(smem + kDqBar);
@@ -597,7 +587,7 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sb = smem_u32(smem);
   if ((sb & 1023u) != 0) {          // the swizzle pattern repeats every 1024 bytes
-    if (threadIdx.x == 0) report_failure(p.status, ST_BAD_ARGUMENT, 499, sb, 1024);
+    if (threadIdx.x == 0 && p.status != nullptr) report_failure(p.status, ST_BAD_ARGUMENT, 499, sb, 1024);
     return;
   }
   KvBars* bars = reinterpret_cast<KvBars*>(smem + kKvBar);
@@ -945,7 +935,7 @@ bool encode_sequences(CUtensorMap* map, const void* base, uint64_t batch, uint64
 size_t attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv_heads, int window) {
   const size_t rows = static_cast<size_t>(batch) * q_heads * ((static_cast<size_t>(seq) + kBlk - 1) / kBlk * kBlk);
   const Runs runs = kv_runs(batch, seq, kv_heads, q_heads / kv_heads, window < seq ? window : 0);
-  return kBwdStatusBytes + 2 * rows * 32 + static_cast<size_t>(runs.count) * 2 * kPartVecs * sizeof(float4);
+  return 2 * rows * 32 + static_cast<size_t>(runs.count) * 2 * kPartVecs * sizeof(float4);
 }
 
 cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream) {
@@ -970,8 +960,7 @@ cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream) {
   p.kv_heads = a.kv_heads;
   p.group = a.q_heads / a.kv_heads;
   p.window = a.window < a.seq ? a.window : 0;     // a window no shorter than the sequence hides nothing
-  // the workspace: a status record for callers without one, the row constants, the parts of cut tiles
-  p.lse2 = static_cast<uint8_t*>(a.workspace) + kBwdStatusBytes;
+  p.lse2 = static_cast<uint8_t*>(a.workspace);
   p.delta = p.lse2 + static_cast<int64_t>(a.batch) * a.q_heads * p.seq_pad * 32;
   p.partial = reinterpret_cast<float4*>(p.delta + static_cast<int64_t>(a.batch) * a.q_heads * p.seq_pad * 32);
   const Runs runs = kv_runs(a.batch, a.seq, a.kv_heads, p.group, p.window);
@@ -982,11 +971,6 @@ cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream) {
   p.cap_in = cap ? 2.0f * kLog2e * a.scale / a.softcap : 0.0f;
   p.cap_out = a.softcap * kLog2e;
   p.status = a.status;
-  if (p.status == nullptr) {
-    p.status = static_cast<Status*>(a.workspace);
-    const cudaError_t zeroed = cudaMemsetAsync(a.workspace, 0, sizeof(Status), stream);
-    if (zeroed != cudaSuccess) return zeroed;
-  }
   const int64_t q_items = static_cast<int64_t>(p.tiles) * a.batch * a.q_heads;
   const int64_t kv_items = static_cast<int64_t>(p.tiles) * a.batch * a.kv_heads;
   auto dq = cap ? attention_bwd_dq_kernel<true> : attention_bwd_dq_kernel<false>;

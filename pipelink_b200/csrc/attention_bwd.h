@@ -28,8 +28,6 @@ struct AttnBwdParams {
   Status* status;
 };
 
-constexpr int kBwdStatusBytes = 256;
-
 struct AttnBwdArgs {
   const void *q, *k, *v, *out, *d_out;
   const float* lse;
@@ -39,7 +37,7 @@ struct AttnBwdArgs {
   float scale, softcap;
   int window;
   int num_sms;
-  Status* status;            // null: one in the workspace, which nobody reads
+  Status* status;            // or null: failures go unreported
 };
 
 size_t attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv_heads, int window);

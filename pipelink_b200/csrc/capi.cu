@@ -1076,7 +1076,7 @@ int plb_rmsnorm_bwd(const void* d_y, int64_t ld_d_y, const void* hidden, int64_t
                     float* d_weight, void* workspace, size_t workspace_bytes, void* stream) {
   if (rows < 0 || width < 1 || rows > 0x7FFFFF00ll || width > 0x7FFFFFFFll || ld_d_y < 0 || ld_hidden < 0 || ld_d_hidden < 0)
     return PLB_E_ARGUMENT;
-  if (!weight || !d_weight || !workspace) return PLB_E_ARGUMENT;
+  if (!weight || !d_weight || !workspace || !aligned16(workspace)) return PLB_E_ARGUMENT;
   if (rows > 0 && (!d_y || !hidden || !rstd || !d_x)) return PLB_E_ARGUMENT;
   if (workspace_bytes < plb_rmsnorm_bwd_workspace_bytes(rows, width)) return PLB_E_CAPACITY;
   plb::NormBwdArgs a;

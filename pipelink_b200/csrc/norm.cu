@@ -57,6 +57,10 @@ struct Chunk<8> {
     const uint32_t w = i < 2 ? raw.x : i < 4 ? raw.y : i < 6 ? raw.z : raw.w;
     return i & 1 ? bf16_hi(w) : bf16_lo(w);
   }
+  __device__ __forceinline__ Pair pair(int i) const {      // numbers 2 i and 2 i + 1
+    const uint32_t w = i == 0 ? raw.x : i == 1 ? raw.y : i == 2 ? raw.z : raw.w;
+    return make_pair(bf16_lo(w), bf16_hi(w));
+  }
   __device__ __forceinline__ void set(const float (&f)[8]) {
     raw = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
   }
@@ -70,6 +74,12 @@ struct Chunk<1> {
   __device__ __forceinline__ float get(int) const { return __bfloat162float(raw); }
   __device__ __forceinline__ void set(const float (&f)[1]) { raw = __float2bfloat16_rn(f[0]); }
 };
+
+// Two by two, the numbers of a thread's chunks: of one chunk, or of two chunks of one.
+template <int NV>
+__device__ __forceinline__ Pair pair_of(const Chunk<8> (&c)[NV], int i) { return c[i >> 2].pair(i & 3); }
+template <int NV>
+__device__ __forceinline__ Pair pair_of(const Chunk<1> (&c)[NV], int i) { return make_pair(c[2 * i].get(0), c[2 * i + 1].get(0)); }
 
 // The SIZE threads of a row: a warp (eight rows a CTA, no barriers) or a whole CTA. A compile-time size: with the
 // exact number of warps a width needs, known at run time only, 16384 x 4096 takes 94 us instead of 91.
@@ -205,30 +215,21 @@ rmsnorm_bwd_rows(const __grid_constant__ NormBwdArgs a) {
   const int width = static_cast<int>(a.width);
   const int64_t sets = (a.rows + Team::kRows - 1) / Team::kRows;
   const float inv_width = 1.0f / static_cast<float>(width);
-  float dw[NV][VEC];
+  constexpr int kPairs = NV * VEC / 2;
+  Pair dw[kPairs];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) dw[i][e] = 0.0f;
+  for (int i = 0; i < kPairs; ++i) dw[i] = make_pair(0.0f, 0.0f);
   // the weight's columns of this thread: kept in registers, or read again (from L1) where those are short
   constexpr bool kKeepWeight = NV * VEC < 32;
-  Chunk<VEC> kept[kKeepWeight ? NV : 1];
-  auto weight = [&](int i) {
-    if constexpr (kKeepWeight) return kept[i];
+  Chunk<VEC> w[NV];
+  auto load_weight = [&](int i) {
     const int c = (t + i * SIZE) * VEC;
-    Chunk<VEC> v;
-    v.zero();
-    if (c < width) v.load(static_cast<const __nv_bfloat16*>(a.weight) + c);
-    return v;
+    w[i].zero();
+    if (c < width) w[i].load(static_cast<const __nv_bfloat16*>(a.weight) + c);
   };
-  if constexpr (kKeepWeight) {
+  if (kKeepWeight)
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * SIZE) * VEC;
-      kept[i].zero();
-      if (c < width) kept[i].load(static_cast<const __nv_bfloat16*>(a.weight) + c);
-    }
-  }
+    for (int i = 0; i < NV; ++i) load_weight(i);
   struct Row { Chunk<VEC> g[NV], h[NV], r[NV]; float rstd; };
   auto fetch = [&](Row& v, int64_t set) {
     const int64_t row = set * Team::kRows + team;
@@ -250,9 +251,9 @@ rmsnorm_bwd_rows(const __grid_constant__ NormBwdArgs a) {
     }
     v.rstd = live ? a.rstd[row] : 0.0f;
   };
-  // a warp that has a row to itself loads the next while it sums this one (65536 x 512: 48 us without, 46 with); CTAs
-  // of several warps do not gain from it
-  constexpr bool kAhead = SIZE == 32 && NV * VEC <= 16;
+  // the next row's loads are in flight while this one is summed, where registers allow (16384 x 4096: 102 us without,
+  // 86 with)
+  constexpr bool kAhead = SIZE <= 512 && NV * VEC <= (VEC == 8 ? 16 : 8);
   Row next;
   if (kAhead) fetch(next, blockIdx.x);
   int round = 0;
@@ -266,58 +267,63 @@ rmsnorm_bwd_rows(const __grid_constant__ NormBwdArgs a) {
     } else {
       fetch(now, set);
     }
-    Chunk<VEC>(&g)[NV] = now.g;
-    Chunk<VEC>(&h)[NV] = now.h;
-    Chunk<VEC>(&r)[NV] = now.r;
     const float rstd = now.rstd;
-    float dot = 0.0f;
+    // n and g of the row in fp32, packed: unpacking the operands once, two numbers to an instruction
+    Pair n[kPairs], gw[kPairs];
+    Pair dot = make_pair(0.0f, 0.0f);
+    const Pair rstd2 = make_pair(rstd, rstd);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const Chunk<VEC> w = weight(i);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float n = h[i].get(e) * rstd;
-        dw[i][e] = fmaf(g[i].get(e), n, dw[i][e]);
-        dot = fmaf(g[i].get(e) * w.get(e), n, dot);
-      }
+    for (int i = 0; i < kPairs; ++i) {
+      if (!kKeepWeight && 2 * i % VEC == 0) load_weight(2 * i / VEC);
+      const Pair g = pair_of(now.g, i);
+      n[i] = mul2(pair_of(now.h, i), rstd2);
+      dw[i] = fma2(g, n[i], dw[i]);
+      gw[i] = mul2(g, pair_of(w, i));
+      dot = fma2(gw[i], n[i], dot);
     }
-    const float mean = Team::sum(dot, round) * inv_width;
+    float dot_lo, dot_hi;
+    split(dot, dot_lo, dot_hi);
+    const float mean = Team::sum(dot_lo + dot_hi, round) * inv_width;
     if (!live) continue;
     __nv_bfloat16* d_x = static_cast<__nv_bfloat16*>(a.d_x) + row * width;
+    const Pair minus_mean = make_pair(-mean, -mean);
+    float d[NV][VEC];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i)
+      split(fma2(fma2(n[i], minus_mean, gw[i]), rstd2, pair_of(now.r, i)), d[2 * i / VEC][2 * i % VEC], d[(2 * i + 1) / VEC][(2 * i + 1) % VEC]);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (t + i * SIZE) * VEC;
       if (c >= width) continue;
-      const Chunk<VEC> w = weight(i);
-      float d[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        d[e] = fmaf(rstd, fmaf(-h[i].get(e) * rstd, mean, g[i].get(e) * w.get(e)), r[i].get(e));
       Chunk<VEC> out;
-      out.set(d);
+      out.set(d[i]);
       out.store(d_x + c);
     }
   }
+  float sums[NV * VEC];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) split(dw[i], sums[2 * i], sums[2 * i + 1]);
   if constexpr (Team::kRows > 1) {                 // the CTA's rows of each column, in their order
     __shared__ float part[kNormThreads][NV * VEC];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) part[threadIdx.x][i * VEC + e] = dw[i][e];
+    for (int i = 0; i < NV * VEC; ++i) part[threadIdx.x][i] = sums[i];
     __syncthreads();
     if (team != 0) return;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        for (int k = 1; k < Team::kRows; ++k) dw[i][e] += part[k * 32 + t][i * VEC + e];
+    for (int i = 0; i < NV * VEC; ++i)
+      for (int k = 1; k < Team::kRows; ++k) sums[i] += part[k * 32 + t][i];
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (t + i * SIZE) * VEC;
     if (c >= width) continue;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) a.workspace[static_cast<int64_t>(blockIdx.x) * width + c + e] = dw[i][e];
+    float* dst = a.workspace + static_cast<int64_t>(blockIdx.x) * width + c;
+    if constexpr (VEC == 8) {
+      reinterpret_cast<float4*>(dst)[0] = make_float4(sums[i * 8], sums[i * 8 + 1], sums[i * 8 + 2], sums[i * 8 + 3]);
+      reinterpret_cast<float4*>(dst)[1] = make_float4(sums[i * 8 + 4], sums[i * 8 + 5], sums[i * 8 + 6], sums[i * 8 + 7]);
+    } else {
+      *dst = sums[i];
+    }
   }
 }
 
@@ -392,7 +398,7 @@ rmsnorm_dw_wide(const NormBwdArgs a, int64_t rows_per_strip) {
 }
 
 // d_weight = sum over the strips: 32 columns a CTA, a strip a warp, the warps' sums joined in their order. 32 warps
-// so that a few loads in flight per thread cover all strips (444 strips of 4096: kSumNote).
+// so that a few loads in flight per thread cover all strips (296 strips of 4096: 3 us; 8 warps took 10).
 constexpr int kSumThreads = 1024;
 __global__ void __launch_bounds__(kSumThreads)
 rmsnorm_dw_sum(const float* __restrict__ partial, int strips, int64_t width, float* __restrict__ d_weight) {
@@ -420,7 +426,7 @@ struct RowShape {
 // Calls f with the row shape for a width, false where rows do not fit in registers. Rows that a warp can hold get a
 // warp, wider ones a CTA of 256 threads as long as those can hold them, and few rows as many threads as they fill,
 // since the time of one row is what counts there (1 x 4096: 2.4 us with 512 threads).
-template <class F>
+template <bool kBack, class F>
 bool by_row_shape(bool vec, int64_t width, bool few, F&& f) {
   if (vec) {
     const int64_t n = width / 8;
@@ -431,7 +437,10 @@ bool by_row_shape(bool vec, int64_t width, bool few, F&& f) {
     else if (few && n <= 512) f(RowShape<8, 512, 1>{});
     else if (few && n <= 1024) f(RowShape<8, 1024, 1>{});
     else if (n <= 512) f(RowShape<8, 256, 2>{});
-    else if (n <= 1024) f(RowShape<8, 256, 4>{});
+    else if (n <= 1024) {
+      if constexpr (kBack) f(RowShape<8, 512, 2>{});          // 32 elements a thread and their sums spill (8192 x 8192: 119 us, so 88)
+      else f(RowShape<8, 256, 4>{});
+    }
     else if (n <= 2048) f(RowShape<8, 512, 4>{});
     else return false;
   } else {
@@ -453,7 +462,7 @@ cudaError_t launch_rmsnorm_fwd(const NormFwdArgs& a, cudaStream_t stream) {
   if (rows == 0) return cudaSuccess;
   const bool vec = a.width % 8 == 0 && a.ld_x % 8 == 0 && a.ld_residual % 8 == 0 && aligned16(a.x) && aligned16(a.residual) &&
                    aligned16(a.weight) && aligned16(a.hidden) && aligned16(a.y);
-  const bool done = by_row_shape(vec, a.width, a.rows <= a.num_sms, [&](auto s) {
+  const bool done = by_row_shape<false>(vec, a.width, a.rows <= a.num_sms, [&](auto s) {
     using S = decltype(s);
     using Team = RowTeam<S::kSize>;
     rmsnorm_fwd_rows<S::kVec, S::kSize, S::kNv><<<static_cast<unsigned>((rows + Team::kRows - 1) / Team::kRows), Team::kThreads, 0, stream>>>(a);
@@ -466,7 +475,7 @@ cudaError_t launch_rmsnorm_bwd(const NormBwdArgs& a, cudaStream_t stream) {
   const bool vec = a.width % 8 == 0 && a.ld_d_y % 8 == 0 && a.ld_hidden % 8 == 0 && a.ld_d_hidden % 8 == 0 && aligned16(a.d_y) &&
                    aligned16(a.hidden) && aligned16(a.d_hidden) && aligned16(a.weight) && aligned16(a.d_x);
   int64_t strips = norm_bwd_strips(a.rows);
-  const bool done = by_row_shape(vec, a.width, a.rows <= a.num_sms, [&](auto s) {
+  const bool done = by_row_shape<true>(vec, a.width, a.rows <= a.num_sms, [&](auto s) {
     using S = decltype(s);
     using Team = RowTeam<S::kSize>;
     const int64_t sets = (a.rows + Team::kRows - 1) / Team::kRows;
