@@ -5,6 +5,9 @@ same ``Shape`` / ``Inputs`` records, the same step order for ``forward`` (schedu
 gate/up GEMM + SwiGLU -> down GEMM + combine placement -> weighted epilogue), the same names for
 the forward-context tensors it returns, and ``ops.mxfp8_quantize`` for weights. All device work
 goes through the C ABI in ``include/pipelink_b200.h``; torch only owns the memory and the stream.
+
+``load_block`` / ``forward_block`` / ``backward_block`` run what a transformer block has in front of its experts (norm with
+the residual's addition, router: ``norm.py``, ``router.py``) together with them; the router's logits are a library product.
 """
 from __future__ import annotations
 
@@ -269,8 +272,12 @@ class MoKHost:
     # ------------------------------------------------------------------ steps
     def schedule_into(self, routes_all_ranks: torch.Tensor):
         """routes: int [world, tokens, topk] (already gathered over the group)."""
-        s, sh = self.schedule, self.shape
         self.routes_i32.copy_(routes_all_ranks.reshape(self.routes_i32.shape))
+        return self.schedule_routes()
+
+    def schedule_routes(self):
+        """The schedule of the routes that already lie in ``routes_i32``."""
+        s, sh = self.schedule, self.shape
         _lib.call("plb_moe_schedule", self.routes_i32.data_ptr(), self.world, sh.tokens, sh.topk,
                   self.rank * self.num_local_experts, self.num_local_experts, self.capacity,
                   self.padding, s.peer_rank.data_ptr(), s.peer_token_idx.data_ptr(),
@@ -286,8 +293,13 @@ class MoKHost:
         rows = self._x_storage.shape[0]
         _lib.call("plb_mxfp8_quantize", self._x_storage.data_ptr(), rows, self.shape.hidden,
                   self.xq.data_ptr(), self.xsc.data_ptr(), None, None, _stream())
+        self.token_scale_rows()
+
+    def token_scale_rows(self):
+        """xsc in the order the bulk-copy dispatch fetches it, where that is the one in use."""
         if self.pull_variant == "bulk" or self.fused_dispatch:
-            _lib.call("plb_ep_scale_rows", self.xsc.data_ptr(), rows, self.shape.hidden, self.xsc_rows.data_ptr(), _stream())
+            _lib.call("plb_ep_scale_rows", self.xsc.data_ptr(), self._x_storage.shape[0], self.shape.hidden,
+                      self.xsc_rows.data_ptr(), _stream())
 
     def pull(self):
         """Dispatch: gather every scheduled row's E4M3 bytes and scale words (comm.cu:105-123)."""
@@ -554,6 +566,79 @@ class MoKHost:
         if check:
             self.status.check("after MoE forward")
         return {"output": out, **self.context_tensors()}
+
+    # ------------------------------------------------------------------ a block's branch: norm, router, experts
+    def load_block(self, norm_weight: torch.Tensor, gate_weight: torch.Tensor, *, gate_bias: torch.Tensor | None = None,
+                   eps: float = 1e-5, **routing):
+        """What stands in front of the experts in a transformer block: the norm's weight bf16 [hidden], the router's
+        bf16 [experts, hidden], its balance bias f32 [experts], and ``router.route_topk``'s score, groups, topk_groups,
+        group_score, renormalize and scale."""
+        sh = self.shape
+        if tuple(norm_weight.shape) != (sh.hidden,) or tuple(gate_weight.shape) != (sh.experts, sh.hidden):
+            raise ValueError("norm and router weights disagree with the session shape")
+        unknown = set(routing) - {"score", "groups", "topk_groups", "group_score", "renormalize", "scale"}
+        if unknown:
+            raise ValueError(f"not an argument of the routing: {', '.join(sorted(unknown))}")
+        on = dict(device=self.device)
+        self.block = dict(norm=norm_weight.to(dtype=torch.bfloat16, **on).contiguous(), eps=float(eps), routing=routing,
+                          gate=gate_weight.to(dtype=torch.bfloat16, **on).contiguous(),
+                          bias=None if gate_bias is None else gate_bias.to(dtype=torch.float32, **on).contiguous(),
+                          hidden=torch.empty((sh.tokens, sh.hidden), dtype=torch.bfloat16, **on),
+                          rstd=torch.empty(sh.tokens, dtype=torch.float32, **on))
+
+    def forward_block(self, x: torch.Tensor, residual: torch.Tensor | None = None, *, check: bool = True, train: bool = False):
+        """The expert branch of a transformer block (single rank): hidden = x + residual, its RMS norm, the router, the
+        experts. x, residual bf16 [tokens, hidden]. The norm writes the tokens as the experts' dispatch takes them (bf16 and,
+        in an MXFP8 session, E4M3 rows and scales) in one launch. Returns ``forward``'s dict with "hidden" (the residual
+        stream, to be the next block's `residual` beside "output" as its x), "experts", "router" and "logits"."""
+        from . import norm, router
+        if self.world != 1:
+            raise ValueError("forward_block() drives one rank")
+        if getattr(self, "block", None) is None or self.weights is None:
+            raise RuntimeError("load_weights() and load_block() first")
+        if train and "w_down_t_fp8" not in self.weights and "w_down_t_bf16" not in self.weights:
+            raise RuntimeError("load_weights(..., train=True) first")
+        blk, mx = self.block, self.precision == "mxfp8"
+        if tuple(x.shape) != (self.shape.tokens, self.shape.hidden):
+            raise ValueError("x disagrees with the session shape")
+        self.status.reset()
+        n = norm.rmsnorm_fwd(x, blk["norm"], residual, eps=blk["eps"], out="both" if mx else "bf16",
+                             into=norm.Normed(blk["hidden"], blk["rstd"], self.x_buffer, self.xq if mx else None, self.xsc if mx else None))
+        blk["stream"] = n.hidden if residual is not None else x
+        if mx:
+            self.token_scale_rows()
+        blk["logits"] = torch.mm(self.x_buffer, blk["gate"].T, out_dtype=torch.float32)
+        router.route_topk(blk["logits"], self.shape.topk, bias=blk["bias"], into=(self.routes_i32, self.router_weight_buffer),
+                          **blk["routing"])
+        self.schedule_routes()
+        self.pull()
+        if train:
+            self.gemm_gate_up_train()
+        else:
+            self.gemm_gate_up()
+        self.gemm_down()
+        out = self.fwd_epilogue()
+        if check:
+            self.status.check("after a block's forward pass")
+        return {"output": out, "hidden": blk["stream"], "experts": self.routes_i32[0], "router": self.router_weight_buffer,
+                "logits": blk["logits"], **self.context_tensors()}
+
+    def backward_block(self, d_out: torch.Tensor, d_hidden: torch.Tensor | None = None, *, check: bool = True, recompute: bool = False):
+        """Backward of the last ``forward_block(train=True)`` (or of a plain one with ``recompute``): `d_out` is the gradient of
+        "output", `d_hidden` what reaches "hidden" from behind. Returns d_x (of x and of the residual alike), d_norm_weight,
+        d_gate_weight (f32) and the experts' gradients as ``backward`` names them."""
+        from . import norm, router
+        blk = getattr(self, "block", None)
+        if blk is None or "logits" not in blk:
+            raise RuntimeError("forward_block() first")
+        g = self.backward(d_out, check=False, recompute=recompute)
+        routing = {k: v for k, v in blk["routing"].items() if k in ("score", "renormalize", "scale")}
+        d_logits = router.route_topk_bwd(g["d_router_weights"], blk["logits"], self.routes_i32[0], **routing)
+        d_y = torch.addmm(g["d_x"].float(), d_logits, blk["gate"].float()).to(torch.bfloat16)
+        d_x, d_norm = norm.rmsnorm_bwd(d_y, blk["stream"], blk["rstd"], blk["norm"], d_hidden)
+        if check:
+            self.status.check("after a block's backward pass")
+        return {**g, "d_x": d_x, "d_norm_weight": d_norm, "d_gate_weight": d_logits.T @ self.x_buffer.float()}
 
     def host_pipeline(self):
         """A forward loop over HOST buffers (see HostPipeline)."""
