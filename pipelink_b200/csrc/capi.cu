@@ -1106,6 +1106,8 @@ int plb_route_topk(const void* logits, int64_t ld_logits, int logits_bf16, const
   a.logits = logits; a.bias = bias; a.tokens = tokens; a.ld_logits = ld_logits;
   a.experts = experts; a.topk = topk; a.groups = topk_groups == groups ? 1 : groups;   // all groups kept: none are told apart
   a.topk_groups = topk_groups == groups ? 1 : topk_groups;
+  a.group_share = 32;
+  while (a.group_share * a.groups > 32) a.group_share >>= 1;
   a.bf16 = logits_bf16 != 0; a.sigmoid = score == 1; a.group_top2 = group_top2 != 0; a.renormalize = renormalize != 0;
   a.scale = scale;
   a.experts_out = experts_out; a.weights_out = weights_out;

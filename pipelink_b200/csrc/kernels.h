@@ -202,6 +202,7 @@ struct RouteArgs {
   const float* bias;         // [experts] or null
   int64_t tokens, ld_logits;
   int experts, topk, groups, topk_groups;
+  int group_share;           // lanes that look through a group: the largest power of two with group_share * groups <= 32
   bool bf16, sigmoid, group_top2, renormalize;
   float scale;
   int* experts_out;          // [tokens, topk]

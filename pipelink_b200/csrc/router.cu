@@ -94,7 +94,7 @@ struct ExactScores {
   }
 };
 
-// The groups a token keeps, from fp64 scores. `choice`: the warp's shared memory, a word per expert.
+// The groups a token keeps (bit g * group_share: group g), from fp64 scores. `choice`: the warp's shared memory, a word per expert.
 __device__ __noinline__ uint32_t exact_groups(const RouteArgs& a, int64_t token, double* choice) {
   const int lane = threadIdx.x & 31, size = a.experts / a.groups;
   const ExactScores s(a, token);
@@ -115,7 +115,10 @@ __device__ __noinline__ uint32_t exact_groups(const RouteArgs& a, int64_t token,
     better += other > mine || (other == mine && g < lane);
   }
   __syncwarp();
-  return __ballot_sync(kAll, lane < a.groups && better < a.topk_groups);
+  const uint32_t groups = __ballot_sync(kAll, lane < a.groups && better < a.topk_groups);
+  uint32_t kept = 0;
+  for (int g = 0; g < a.groups; ++g) kept |= ((groups >> g) & 1u) << (g * a.group_share);
+  return kept;
 }
 
 // Lanes 0 .. count - 1 hold candidates, among them all that may be chosen: in their order by fp64 choice values.
@@ -142,7 +145,7 @@ __device__ __noinline__ int exact_choice(const RouteArgs& a, int64_t token, uint
   const int lane = threadIdx.x & 31, size = a.experts / a.groups;
   const ExactScores s(a, token);
   __syncwarp();
-  for (int e = lane; e < a.experts; e += 32) key[e] = !((kept >> (a.groups > 1 ? e / size : 0)) & 1u) ? 0 : order_key(s.choice(e));
+  for (int e = lane; e < a.experts; e += 32) key[e] = !((kept >> (a.groups > 1 ? e / size * a.group_share : 0)) & 1u) ? 0 : order_key(s.choice(e));
   __syncwarp();
   int pick = 0;
   for (int j = 0; j < a.topk; ++j) {
@@ -163,8 +166,10 @@ __device__ __noinline__ int exact_choice(const RouteArgs& a, int64_t token, uint
   return pick;
 }
 
+// CTAs per SM: what hides the latencies of a token's steps is other tokens, at the price of registers where a lane
+// holds few experts (256 experts in groups: 32 us with 24 warps an SM, 27 with 48).
 template <int NV>
-__global__ void __launch_bounds__(kRouteWarps * 32)
+__global__ void __launch_bounds__(kRouteWarps * 32, NV <= 8 ? 12 : NV <= 16 ? 8 : 4)
 route_topk_kernel(const __grid_constant__ RouteArgs a) {
   extern __shared__ uint64_t shared[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -193,12 +198,12 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
     sum = warp_sum(sum);
     inv_sum = sum == 0.0f ? 0.0f : 1.0f / sum;
   }
-  auto score = [&](float x) { return a.sigmoid ? 1.0f / (1.0f + expf(-x)) : expf(x - top) * inv_sum; };
+  auto score = [&](float x) { return a.sigmoid ? __fdividef(1.0f, 1.0f + expf(-x)) : expf(x - top) * inv_sum; };
   // How far two fp32 choice values must lie apart to be in the order of the exact ones: twice the error of a score,
-  // and the roundings of the sums (under 2^-23 of |c| + 1/4 each). A sigmoid is off by the step of expf (2^-23), the
-  // sum's and the quotient's half steps: 2^-22 at most. A softmax by two steps of expf, the sum's NV + 5 roundings, two
+  // and the roundings of the sums (under 2^-23 of |c| + 1/4 each). A sigmoid is off by the two steps of expf (2^-23
+  // each), the sum's half step and the quotient's two: 2^-20.8 at most. A softmax by two steps of expf, the sum's NV + 5 roundings, two
   // more, and half a step of |x - top|, which is largest against exp(top - x) at 1: under (NV + 12) 2^-23 of the largest.
-  const float slack = a.sigmoid ? 4.8e-7f : (NV + 12) * 2.4e-7f * inv_sum;
+  const float slack = a.sigmoid ? 1.1e-6f : (NV + 12) * 2.4e-7f * inv_sum;
   auto near = [&](float high, float low) { return high - low <= slack + 2.4e-7f * (fabsf(high) + 0.25f); };   // NaN and inf - inf: not near
   if (by_score || by_sum) {
 #pragma unroll
@@ -210,23 +215,23 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
       if (by_score) key[i] = order_key(c[i]);
     }
   }
-  uint32_t kept = kAll;
+  uint32_t kept = kAll;                                           // bit g * share: group g takes part
   if (a.groups > 1) {
     // `share` adjacent lanes look through a group; in shared memory each group starts `share` words on, so that the
     // groups' lanes meet different banks
     const int size = a.experts / a.groups;
     const float inv_size = 1.0f / static_cast<float>(size);
-    auto group_of = [&](int e) { return static_cast<int>((static_cast<float>(e) + 0.5f) * inv_size); };   // exact up to 1024
-    int share = 32;
-    while (share * a.groups > 32) share >>= 1;
+    const int share = a.group_share, log_share = 31 - __clz(share);
     float* choice = reinterpret_cast<float*>(scratch);
+    int first_lane[NV];                                            // of an expert's group
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int e = lane + 32 * i;
-      if (e < a.experts) choice[e + group_of(e) * share] = c[i];
+      first_lane[i] = static_cast<int>((static_cast<float>(e) + 0.5f) * inv_size) << log_share;      // the quotient is exact up to 1024
+      if (e < a.experts) choice[e + first_lane[i]] = c[i];
     }
     __syncwarp();
-    const int g = lane / share, sub = lane - g * share;
+    const int g = lane >> log_share, sub = lane & (share - 1);
     float first = -INFINITY, second = -INFINITY;
     if (g < a.groups)
       for (int e = sub; e < size; e += share) {
@@ -242,13 +247,11 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
     const uint32_t mine = order_key(by_sum && second > -INFINITY ? first + second : first);
     int better = 0;
     for (int h = 0; h < a.groups; ++h) {
-      const uint32_t other = __shfl_sync(kAll, mine, h * share);
+      const uint32_t other = __shfl_sync(kAll, mine, h << log_share);
       better += other > mine || (other == mine && h < g);
     }
     const bool keep = g < a.groups && better < a.topk_groups;
-    kept = 0;
-    const uint32_t lanes = __ballot_sync(kAll, keep);
-    for (int h = 0; h < a.groups; ++h) kept |= ((lanes >> (h * share)) & 1u) << h;
+    kept = __ballot_sync(kAll, keep);
     if (by_score || by_sum) {
       const uint32_t worst_kept = __reduce_min_sync(kAll, keep ? mine : 0xFFFFFFFFu);
       const uint32_t best_dropped = __reduce_max_sync(kAll, g < a.groups && !keep ? mine : 0u);
@@ -257,7 +260,7 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (lane + 32 * i < a.experts && !((kept >> group_of(lane + 32 * i)) & 1u)) key[i] = 0;
+      if (lane + 32 * i < a.experts && !((kept >> first_lane[i]) & 1u)) key[i] = 0;
   }
   uint32_t best = 0;     // this lane's best candidate and its register
   int slot = 0;

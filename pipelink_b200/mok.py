@@ -66,8 +66,10 @@ def dense(t: torch.Tensor) -> torch.Tensor:
 
 
 def rows_of(t: torch.Tensor):
-    """[..., width] as 2-D rows of unit-stride elements and their stride: a view where one exists (a slice of a wider
+    """[..., width] as rows of unit-stride elements and their stride: a view where one exists (a slice of a wider
     tensor, a broadcast row), a copy otherwise."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
     if t.stride(1) != 1 and t.shape[1] > 1:
         t = t.contiguous()
