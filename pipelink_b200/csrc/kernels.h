@@ -204,6 +204,7 @@ struct RouteArgs {
   int experts, topk, groups, topk_groups;
   int group_share;           // lanes that look through a group: the largest power of two with group_share * groups <= 32
   bool bf16, sigmoid, group_top2, renormalize;
+  bool wide;                 // set by the launcher: lanes load whole pieces of a row
   float scale;
   int* experts_out;          // [tokens, topk]
   float* weights_out;
@@ -215,6 +216,7 @@ struct RouteBwdArgs {
   int64_t tokens, ld_logits;
   int experts, topk;
   bool bf16, sigmoid, renormalize;
+  bool wide, wide_out;       // set by the launcher
   float scale;
   void* d_logits;            // [tokens, experts], the logits' type
 };

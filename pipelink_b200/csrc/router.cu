@@ -5,7 +5,7 @@
 //   the topk best c of the kept groups, ties to the lowest index; w = scale * s [/ sum of the chosen s]
 //   dS_j = scale / S * (g_j - sum_i g_i s_i / S) or scale * g_j;  dx = s (dS - sum s dS) or dS s (1 - s)
 //
-// One warp per token, expert e in register e / 32 of lane e % 32. The topk-th largest of the 32 lanes' maxima bounds
+// One warp per token, NV consecutive experts to a lane. The topk-th largest of the 32 lanes' maxima bounds
 // the topk-th value from below: what is not under it, some 10 to 20 candidates, is put one to a lane and ranked by
 // comparing each with each (16384 tokens, 256 experts, 8 chosen: kRouteNote). Where that leaves more than 32 (many
 // ties, a large topk), topk rounds of a warp-wide maximum choose. Without a bias the scores are ordered as the logits are, and those are compared as they
@@ -26,8 +26,49 @@ constexpr int kRouteWarps = 4;
 constexpr uint32_t kAll = 0xFFFFFFFFu;
 constexpr int kMostRanked = 16;       // topk up to which the lanes' maxima leave few candidates
 
+// A warp's shared memory: a word per expert and 32 more, in 16-byte pieces.
+__host__ __device__ constexpr int scratch_words(int experts) { return (experts + 33) & ~1; }
+
 __device__ __forceinline__ float load_logit(const void* p, int64_t i, bool bf16) {
   return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];
+}
+// A lane's NV consecutive logits (of the row at index `row`); past the experts -inf. Whole rows in 16-byte pieces where
+// `wide`: row starts and lengths are multiples of a lane's share.
+template <int NV>
+__device__ __forceinline__ void load_logits(const void* p, int64_t row, int experts, bool bf16, bool wide, float (&x)[NV]) {
+  const int first = (threadIdx.x & 31) * NV;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) x[i] = -INFINITY;
+  if (first >= experts) return;
+  if (!wide) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (first + i < experts) x[i] = load_logit(p, row + first + i, bf16);
+  } else if (bf16) {
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p) + row + first);
+    uint32_t w[NV / 2];
+    if constexpr (NV == 2) w[0] = *q;
+    else if constexpr (NV == 4) { const uint2 v = *reinterpret_cast<const uint2*>(q); w[0] = v.x; w[1] = v.y; }
+    else {
+#pragma unroll
+      for (int i = 0; i < NV / 8; ++i) {
+        const uint4 v = reinterpret_cast<const uint4*>(q)[i];
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV / 2; ++i) { x[2 * i] = bf16_lo(w[i]); x[2 * i + 1] = bf16_hi(w[i]); }
+  } else {
+    const float* q = static_cast<const float*>(p) + row + first;
+    if constexpr (NV == 2) { const float2 v = *reinterpret_cast<const float2*>(q); x[0] = v.x; x[1] = v.y; }
+    else {
+#pragma unroll
+      for (int i = 0; i < NV / 4; ++i) {
+        const float4 v = reinterpret_cast<const float4*>(q)[i];
+        x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+      }
+    }
+  }
 }
 // Unsigned integers in the order of the numbers; NaN below every number, 0 is left for "not a candidate".
 __device__ __forceinline__ uint64_t order_key(double v) {
@@ -39,6 +80,7 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t b = __float_as_uint(v + 0.0f);            // -0 becomes 0
   return v != v ? 1u : b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
+constexpr uint32_t kMasked = 0x007FFFFFu;                   // the key of -inf
 __device__ __forceinline__ float key_value(uint32_t k) {   // the number of a key that is one
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
@@ -62,7 +104,7 @@ __device__ __forceinline__ T warp_max(T v) {
 __device__ __forceinline__ void store_choice(const RouteArgs& a, int64_t token, int lane, int pick, float weight) {
   if (a.renormalize) {
     const float total = warp_sum(lane < a.topk ? weight : 0.0f);
-    weight = total == 0.0f ? 0.0f : weight / total;
+    weight = total == 0.0f ? 0.0f : __fdividef(weight, total);
   }
   if (lane < a.topk) {
     a.experts_out[token * a.topk + lane] = pick;
@@ -171,19 +213,19 @@ __device__ __noinline__ int exact_choice(const RouteArgs& a, int64_t token, uint
 template <int NV>
 __global__ void __launch_bounds__(kRouteWarps * 32, NV <= 8 ? 12 : NV <= 16 ? 8 : 4)
 route_topk_kernel(const __grid_constant__ RouteArgs a) {
-  extern __shared__ uint64_t shared[];
+  extern __shared__ __align__(16) uint64_t shared[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t token = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
   if (token >= a.tokens) return;
-  uint64_t* scratch = shared + warp * (a.experts + 32);
-  float c[NV];           // logits, then what a choice goes by
+  uint64_t* scratch = shared + warp * scratch_words(a.experts);
+  const int e0 = lane * NV;              // the lane's first expert
+  float c[NV];                           // logits, then what a choice goes by
   uint32_t key[NV];
   float top = -INFINITY;
+  load_logits<NV>(a.logits, token * a.ld_logits, a.experts, a.bf16, a.wide, c);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int e = lane + 32 * i;
-    c[i] = e < a.experts ? load_logit(a.logits, token * a.ld_logits + e, a.bf16) : -INFINITY;
-    key[i] = e < a.experts ? order_key(c[i]) : 0;
+    key[i] = e0 + i < a.experts ? order_key(c[i]) : 0;
     top = fmaxf(top, c[i]);
   }
   const bool by_score = a.bias != nullptr;                        // else by logits
@@ -194,51 +236,56 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
     if (top == -INFINITY) top = 0.0f;
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) sum += expf(c[i] - top);
+    for (int i = 0; i < NV; ++i) {
+      const float e = expf(c[i] - top);
+      sum += e;
+      if (by_score || by_sum) c[i] = e;
+    }
     sum = warp_sum(sum);
-    inv_sum = sum == 0.0f ? 0.0f : 1.0f / sum;
+    inv_sum = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
   }
   auto score = [&](float x) { return a.sigmoid ? __fdividef(1.0f, 1.0f + expf(-x)) : expf(x - top) * inv_sum; };
   // How far two fp32 choice values must lie apart to be in the order of the exact ones: twice the error of a score,
   // and the roundings of the sums (under 2^-23 of |c| + 1/4 each). A sigmoid is off by the two steps of expf (2^-23
-  // each), the sum's half step and the quotient's two: 2^-20.8 at most. A softmax by two steps of expf, the sum's NV + 5 roundings, two
-  // more, and half a step of |x - top|, which is largest against exp(top - x) at 1: under (NV + 12) 2^-23 of the largest.
-  const float slack = a.sigmoid ? 1.1e-6f : (NV + 12) * 2.4e-7f * inv_sum;
+  // each), the sum's half step and the quotient's two: 2^-20.8 at most. A softmax by two steps of expf, the sum's NV + 5 roundings, six
+  // more, and half a step of |x - top|, which is largest against exp(top - x) at 1: under (NV + 16) 2^-23 of the largest.
+  const float slack = a.sigmoid ? 1.1e-6f : (NV + 16) * 2.4e-7f * inv_sum;
   auto near = [&](float high, float low) { return high - low <= slack + 2.4e-7f * (fabsf(high) + 0.25f); };   // NaN and inf - inf: not near
   if (by_score || by_sum) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int e = lane + 32 * i;
-      if (e >= a.experts) continue;
-      const float s = score(c[i]);
-      c[i] = c[i] == -INFINITY ? c[i] : by_score ? s + a.bias[e] : s;
+      if (e0 + i >= a.experts) continue;
+      const float s = a.sigmoid ? score(c[i]) : c[i] * inv_sum;
+      c[i] = key[i] == kMasked ? -INFINITY : by_score ? s + a.bias[e0 + i] : s;
       if (by_score) key[i] = order_key(c[i]);
     }
   }
   uint32_t kept = kAll;                                           // bit g * share: group g takes part
   if (a.groups > 1) {
-    // `share` adjacent lanes look through a group; in shared memory each group starts `share` words on, so that the
-    // groups' lanes meet different banks
-    const int size = a.experts / a.groups;
-    const float inv_size = 1.0f / static_cast<float>(size);
-    const int share = a.group_share, log_share = 31 - __clz(share);
-    float* choice = reinterpret_cast<float*>(scratch);
-    int first_lane[NV];                                            // of an expert's group
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = lane + 32 * i;
-      first_lane[i] = static_cast<int>((static_cast<float>(e) + 0.5f) * inv_size) << log_share;      // the quotient is exact up to 1024
-      if (e < a.experts) choice[e + first_lane[i]] = c[i];
-    }
-    __syncwarp();
-    const int g = lane >> log_share, sub = lane & (share - 1);
+    const int size = a.experts / a.groups, log_share = 31 - __clz(a.group_share), share = a.group_share;
     float first = -INFINITY, second = -INFINITY;
-    if (g < a.groups)
-      for (int e = sub; e < size; e += share) {
-        const float v = choice[g * (size + share) + e];
-        second = fmaxf(second, fminf(first, v));     // fminf, fmaxf pass NaN over
-        first = fmaxf(first, v);
+    auto take = [&](float v) {
+      second = fmaxf(second, fminf(first, v));                    // fminf, fmaxf pass NaN over
+      first = fmaxf(first, v);
+    };
+    const int g = lane >> log_share;
+    if (share * NV == size) {                                     // a group is `share` lanes' registers
+#pragma unroll
+      for (int i = 0; i < NV; ++i) take(c[i]);
+    } else {
+      // `share` adjacent lanes look through a group in shared memory, where each group starts `share` words on, so that
+      // the groups' lanes meet different banks
+      float* choice = reinterpret_cast<float*>(scratch);
+      const float inv_size = 1.0f / static_cast<float>(size);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int e = e0 + i;
+        if (e < a.experts) choice[e + (static_cast<int>((static_cast<float>(e) + 0.5f) * inv_size) << log_share)] = c[i];
       }
+      __syncwarp();
+      if (g < a.groups)
+        for (int e = lane & (share - 1); e < size; e += share) take(choice[g * (size + share) + e]);
+    }
     for (int o = 1; o < share; o <<= 1) {
       const float f = __shfl_xor_sync(kAll, first, o), h = __shfl_xor_sync(kAll, second, o);
       second = fmaxf(fmaxf(second, h), fminf(first, f));
@@ -258,15 +305,22 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
       // sums of two have twice the error
       if (near(key_value(worst_kept) * 0.5f, key_value(best_dropped) * 0.5f)) kept = exact_groups(a, token, reinterpret_cast<double*>(scratch));
     }
+    if (share * NV == size) {
+      if (!((kept >> (g << log_share)) & 1u))
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (lane + 32 * i < a.experts && !((kept >> first_lane[i]) & 1u)) key[i] = 0;
+        for (int i = 0; i < NV; ++i) key[i] = 0;
+    } else {
+      const float inv_size = 1.0f / static_cast<float>(size);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {        // (e + 1/2) / size is exact enough up to 1024
+        const int of = static_cast<int>((static_cast<float>(e0 + i) + 0.5f) * inv_size);
+        if (e0 + i < a.experts && !((kept >> (of << log_share)) & 1u)) key[i] = 0;
+      }
+    }
   }
-  uint32_t best = 0;     // this lane's best candidate and its register
-  int slot = 0;
+  uint32_t best = 0;                       // the lane's best candidate
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (key[i] > best) { best = key[i]; slot = i; }
+  for (int i = 0; i < NV; ++i) best = max(best, key[i]);
   int pick = 0;          // lane j: the j-th candidate, best first
   int count = 33;
   bool close = false;
@@ -283,29 +337,40 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
       if (low == low) bound = order_key(low);
     }
     if (bound == 0) bound = 1;
-    uint32_t* list = reinterpret_cast<uint32_t*>(scratch);           // keys, then experts
-    int n = 0;
-    __syncwarp();
+    uint32_t* list = reinterpret_cast<uint32_t*>(scratch);           // 32 keys, then their experts
+    int mine_in = 0, n = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const bool in = key[i] >= bound;
-      const uint32_t lanes = __ballot_sync(kAll, in);
-      const int at = n + __popc(lanes & ((1u << lane) - 1u));
-      if (in && at < 32) {
-        list[at] = key[i];
-        list[32 + at] = lane + 32 * i;
-      }
-      n += __popc(lanes);
+    for (int i = 0; i < NV; ++i) mine_in += key[i] >= bound;
+    int at = mine_in;                                                // where the lane's candidates go
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int before = __shfl_up_sync(kAll, at, o);
+      if (lane >= o) at += before;
     }
-    __syncwarp();
+    n = __shfl_sync(kAll, at, 31);
     if (n <= 32) {
+      at -= mine_in;
+      __syncwarp();
+      list[lane] = 0;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (key[i] >= bound) {
+          list[at] = key[i];
+          list[32 + at] = e0 + i;
+          ++at;
+        }
+      __syncwarp();
       // the list is in the order of the experts, so among equal keys the earlier place is the lower index
       const uint32_t mine = lane < n ? list[lane] : 0;
       const int e = lane < n ? list[32 + lane] : 0;
       int rank = 0;
-      for (int j = 0; j < n; ++j) {
-        const uint32_t other = list[j];
-        rank += other > mine || (other == mine && j < lane);
+      for (int j = 0; j < n; j += 4) {
+        const uint4 other = *reinterpret_cast<const uint4*>(list + j);
+        rank += other.x + (j < lane) > mine;                         // no key is 2^32 - 1
+        rank += other.y + (j + 1 < lane) > mine;
+        rank += other.z + (j + 2 < lane) > mine;
+        rank += other.w + (j + 3 < lane) > mine;
       }
       __syncwarp();
       if (lane < n) {
@@ -329,8 +394,16 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
     }
   }
   if (count > 32) {
-    uint32_t last = 0;     // the key chosen before, and its expert
+    int slot = 0;          // of the lane's best, and the key chosen before with its expert
+    uint32_t last = 0;
     int last_at = 0;
+    auto look = [&]() {
+      best = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (key[i] > best) { best = key[i]; slot = i; }
+    };
+    look();
     for (count = 0;; ++count) {
       const uint32_t m = __reduce_max_sync(kAll, best);
       // past topk as long as a candidate may still change places with a chosen one
@@ -339,19 +412,16 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
         if (follows) count = 33;
         break;
       }
-      const int at = __reduce_min_sync(kAll, best == m ? lane + 32 * slot : 0x7FFFFFFF);
+      const int at = __reduce_min_sync(kAll, best == m ? e0 + slot : 0x7FFFFFFF);
       if (follows)
         close = close || a.bias[at] != a.bias[last_at] ||
                 load_logit(a.logits, token * a.ld_logits + at, a.bf16) != load_logit(a.logits, token * a.ld_logits + last_at, a.bf16);
       last = m;
       last_at = at;
-      if (lane == (at & 31)) {
-        best = 0;
+      if (lane == at / NV) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          key[i] = at == lane + 32 * i ? 0 : key[i];
-          if (key[i] > best) { best = key[i]; slot = i; }
-        }
+        for (int i = 0; i < NV; ++i) key[i] = at == e0 + i ? 0 : key[i];
+        look();
       }
       if (lane == count) pick = at;
     }
@@ -368,14 +438,12 @@ route_topk_bwd_kernel(const __grid_constant__ RouteBwdArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t token = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
   if (token >= a.tokens) return;
+  const int e0 = lane * NV;
   float s[NV];
   float top = -INFINITY;
+  load_logits<NV>(a.logits, token * a.ld_logits, a.experts, a.bf16, a.wide, s);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = lane + 32 * i;
-    s[i] = e < a.experts ? load_logit(a.logits, token * a.ld_logits + e, a.bf16) : -INFINITY;
-    top = fmaxf(top, s[i]);
-  }
+  for (int i = 0; i < NV; ++i) top = fmaxf(top, s[i]);
   top = warp_max(top);
   if (top == -INFINITY) top = 0.0f;
   float sum = 0.0f;
@@ -403,12 +471,16 @@ route_topk_bwd_kernel(const __grid_constant__ RouteBwdArgs a) {
     g = !valid || total == 0.0f ? 0.0f : (g - inner / total) / total;
   }
   const float dot = a.sigmoid ? 0.0f : warp_sum(g * mine);
-  // slots to experts, in the slots' order (an expert may be named twice)
-  float* ds = ds_all + warp * a.experts;
-  for (int e = lane; e < a.experts; e += 32) ds[e] = 0.0f;
+  // slots to experts, in the slots' order (an expert may be named twice, which the slots' numbers find out)
+  float* ds = ds_all + warp * 32 * NV;
+  int* tag = reinterpret_cast<int*>(ds);
+  if (valid) tag[at] = lane;
   __syncwarp();
-  const uint32_t peers = __match_any_sync(kAll, valid ? at : -1 - lane);
-  const bool alone = __all_sync(kAll, peers == 1u << lane);
+  const bool alone = __all_sync(kAll, !valid || tag[at] == lane);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < NV; ++i) ds[e0 + i] = 0.0f;
+  __syncwarp();
   if (alone) {
     if (valid) ds[at] = g;
   } else {
@@ -419,13 +491,35 @@ route_topk_bwd_kernel(const __grid_constant__ RouteBwdArgs a) {
   }
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = lane + 32 * i;
-    if (e >= a.experts) continue;
-    const float d = a.sigmoid ? ds[e] * s[i] * (1.0f - s[i]) : s[i] * (ds[e] - dot);
-    const int64_t o = token * a.experts + e;
-    if (a.bf16) static_cast<__nv_bfloat16*>(a.d_logits)[o] = __float2bfloat16_rn(d);
-    else static_cast<float*>(a.d_logits)[o] = d;
+  for (int i = 0; i < NV; ++i) s[i] = a.sigmoid ? ds[e0 + i] * s[i] * (1.0f - s[i]) : s[i] * (ds[e0 + i] - dot);
+  if (e0 >= a.experts) return;
+  const int64_t out = token * a.experts + e0;
+  if (a.bf16) {
+    __nv_bfloat16* d = static_cast<__nv_bfloat16*>(a.d_logits) + out;
+    if (a.wide_out) {
+#pragma unroll
+      for (int i = 0; i < NV / 2; ++i) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(s[2 * i], s[2 * i + 1]);
+        reinterpret_cast<__nv_bfloat162*>(d)[i] = v;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (e0 + i < a.experts) d[i] = __float2bfloat16_rn(s[i]);
+    }
+  } else {
+    float* d = static_cast<float*>(a.d_logits) + out;
+    if (a.wide_out) {
+      if constexpr (NV == 2) *reinterpret_cast<float2*>(d) = make_float2(s[0], s[1]);
+      else {
+#pragma unroll
+        for (int i = 0; i < NV / 4; ++i) reinterpret_cast<float4*>(d)[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (e0 + i < a.experts) d[i] = s[i];
+    }
   }
 }
 
@@ -443,18 +537,33 @@ cudaError_t by_width(int experts, F&& f) {
 
 }  // namespace
 
-cudaError_t launch_route_topk(const RouteArgs& a, cudaStream_t stream) {
+// Rows of `experts` numbers from p on, `ld` apart, whose lanes' shares are whole, aligned pieces.
+static bool whole_pieces(const void* p, int64_t ld, int experts, int nv, bool bf16) {
+  const int bytes = nv * (bf16 ? 2 : 4);
+  return experts % nv == 0 && ld % nv == 0 && reinterpret_cast<uintptr_t>(p) % (bytes < 16 ? bytes : 16) == 0;
+}
+
+cudaError_t launch_route_topk(const RouteArgs& args, cudaStream_t stream) {
+  RouteArgs a = args;
   if (a.tokens == 0) return cudaSuccess;
   const unsigned grid = static_cast<unsigned>((a.tokens + kRouteWarps - 1) / kRouteWarps);
   return by_width(a.experts, [&](auto n) {
-    route_topk_kernel<decltype(n)::value><<<grid, kRouteWarps * 32, kRouteWarps * (a.experts + 32) * sizeof(uint64_t), stream>>>(a);
+    constexpr int kNv = decltype(n)::value;
+    a.wide = whole_pieces(a.logits, a.ld_logits, a.experts, kNv, a.bf16);
+    route_topk_kernel<kNv><<<grid, kRouteWarps * 32, kRouteWarps * scratch_words(a.experts) * sizeof(uint64_t), stream>>>(a);
   });
 }
 
-cudaError_t launch_route_topk_bwd(const RouteBwdArgs& a, cudaStream_t stream) {
+cudaError_t launch_route_topk_bwd(const RouteBwdArgs& args, cudaStream_t stream) {
+  RouteBwdArgs a = args;
   if (a.tokens == 0) return cudaSuccess;
   const unsigned grid = static_cast<unsigned>((a.tokens + kRouteWarps - 1) / kRouteWarps);
-  return by_width(a.experts, [&](auto n) { route_topk_bwd_kernel<decltype(n)::value><<<grid, kRouteWarps * 32, kRouteWarps * a.experts * sizeof(float), stream>>>(a); });
+  return by_width(a.experts, [&](auto n) {
+    constexpr int kNv = decltype(n)::value;
+    a.wide = whole_pieces(a.logits, a.ld_logits, a.experts, kNv, a.bf16);
+    a.wide_out = whole_pieces(a.d_logits, a.experts, a.experts, kNv, a.bf16);
+    route_topk_bwd_kernel<kNv><<<grid, kRouteWarps * 32, kRouteWarps * 32 * kNv * sizeof(float), stream>>>(a);
+  });
 }
 
 }  // namespace plb
