@@ -32,7 +32,7 @@ using namespace attn;
 
 namespace {
 
-constexpr int kBwdThreads = 384;      // warp 0 TMA, warp 1 MMA, warps 4-11 compute
+constexpr int kBwdThreads = 384;      // warp 0 TMA, warp 1 MMA, warps 2-3 the rows' constants (dq), warps 4-11 compute
 constexpr int kComputeWarps = 8;
 constexpr uint32_t kFullMask = 0xFFFFFFFFu;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -41,8 +41,9 @@ constexpr int kBwdRuns = 148;         // runs of steps: a CTA on every SM; no ru
 // ---- shared-memory maps (offsets from a 1024-byte aligned base)
 constexpr int kDqK = 2 * kTileBytes, kDqKStages = 3;                  // after Q and dO
 constexpr int kDqV = kDqK + kDqKStages * kTileBytes, kDqVStages = 2;
-constexpr int kDqRed = kDqV + kDqVStages * kTileBytes;                // [2][2][128] floats
-constexpr int kDqBar = kDqRed + 2048;
+constexpr int kDqStat = kDqV + kDqVStages * kTileBytes;               // [2][2][128] floats: log-sum-exp and delta of two tiles
+constexpr int kDqRed = kDqStat + 2048;                                // [128] floats
+constexpr int kDqBar = kDqRed + 512;
 constexpr int kDqSmem = kDqBar + 256;
 
 // dK, dV: K and V, then the streamed tiles with their rows' constants behind them (see kAuxBytes)
@@ -57,7 +58,7 @@ static_assert(kDqSmem <= 232448 && kKvSmem <= 232448, "227 KB of shared memory p
 
 struct DqBars {
   uint64_t q_full, q_empty, k_full[kDqKStages], k_empty[kDqKStages], v_full[kDqVStages], v_empty[kDqVStages];
-  uint64_t s_full[2], dp_full, dp_read, ds_full, dq_full, dq_free, red, drain;
+  uint64_t s_full[2], dp_full, dp_read, ds_full, dq_full, dq_free, red, stat_full[2], stat_empty[2], drain;
   uint32_t tmem_base, pad;
 };
 struct KvBars {
@@ -72,7 +73,10 @@ __device__ __forceinline__ int snake(int wave) {
   return wave * gridDim.x + ((wave & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
-struct DqItem { int b, h, q0, first, blocks; };
+// A tile of queries that see one or two key tiles (`measure`) goes over them twice, first for delta = sum P dP: where a
+// row sees few keys the rounding of the saved output is not averaged out of delta = sum dO O, and with it the error of
+// dQ and dK would be half as large again (sequences of 77: 2.6e-3 of the norm instead of 2.4e-3).
+struct DqItem { int b, h, q0, first, blocks, steps; bool measure; };
 __device__ __forceinline__ DqItem dq_item(const AttnBwdParams& p, int w) {
   const int bh = p.batch * p.q_heads;
   DqItem t;
@@ -83,6 +87,8 @@ __device__ __forceinline__ DqItem dq_item(const AttnBwdParams& p, int w) {
   t.q0 = qb * kBlk;
   t.first = p.window > 0 ? max(0, (t.q0 - p.window + 1) / kBlk) : 0;
   t.blocks = qb + 1 - t.first;
+  t.measure = t.blocks <= 2;
+  t.steps = t.measure ? 2 * t.blocks : t.blocks;
   return t;
 }
 // Query tiles that see key tile kb.
@@ -356,6 +362,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     mbar_init(BAR(dq_full), 1);
     mbar_init(BAR(dq_free), kComputeWarps);
     mbar_init(BAR(red), kComputeWarps);
+    for (int s = 0; s < 2; ++s) { mbar_init(BAR(stat_full) + 8 * s, 2); mbar_init(BAR(stat_empty) + 8 * s, kComputeWarps); }
     mbar_init(BAR(drain), 1);
     fence_mbar_init();
     prefetch_tensormap(&map_q);
@@ -390,8 +397,8 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       }
       __syncwarp();
       ++it;
-      for (int j = 0; j < t.blocks; ++j, ++kv) {
-        const int row = (t.first + j) * kBlk;
+      for (int j = 0; j < t.steps; ++j, ++kv) {
+        const int row = (t.first + (j < t.blocks ? j : j - t.blocks)) * kBlk;
         const uint32_t ks = kv % kDqKStages, vs = kv % kDqVStages;
         if (!warp_wait(BAR(k_empty) + 8 * ks, ((kv / kDqKStages) & 1u) ^ 1u, p.status, ST_TIMEOUT_EMPTY, 401)) { ok = false; break; }
         if (elect_one_sync()) {
@@ -429,7 +436,8 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     for (int wave = 0; ok && wave * static_cast<int>(gridDim.x) < items; ++wave) {
       const int w = snake(wave);
       if (w >= items) continue;
-      const int n = __shfl_sync(kFullMask, dq_item(p, w).blocks, 0);
+      const DqItem t = dq_item(p, w);
+      const int n = __shfl_sync(kFullMask, t.steps, 0), from = __shfl_sync(kFullMask, t.steps - t.blocks, 0);
       if (!warp_wait(BAR(q_full), it & 1u, p.status, ST_TIMEOUT_FULL, 412)) { ok = false; break; }
       tc_fence_after();
       if (!issue_s(blk) || !issue_dp(blk) || (n > 1 && !issue_s(blk + 1))) { ok = false; break; }
@@ -439,10 +447,11 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         if (j + 1 < n && !issue_dp(blk + 1)) { ok = false; break; }
         if (j + 2 == n) warp_commit(BAR(q_empty));       // the last products that read Q and dO are issued: both may be replaced
         if (!warp_wait(BAR(ds_full), blk & 1u, p.status, ST_TIMEOUT_FULL, 413)) { ok = false; break; }
-        if (j == 0 && !warp_wait(BAR(dq_free), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_TMEM_EMPTY, 414)) { ok = false; break; }
+        if (j == from && !warp_wait(BAR(dq_free), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_TMEM_EMPTY, 414)) { ok = false; break; }
         tc_fence_after();
         const uint32_t ks = blk % kDqKStages;
-        mma_from_tmem(t_dq, t_s + (blk & 1u) * 128, sb + kDqK + ks * kTileBytes, j != 0, BAR(k_empty) + 8 * ks);
+        if (j < from) warp_commit(BAR(k_empty) + 8 * ks);
+        else mma_from_tmem(t_dq, t_s + (blk & 1u) * 128, sb + kDqK + ks * kTileBytes, j != from, BAR(k_empty) + 8 * ks);
         if (j + 2 < n && !issue_s(blk + 2)) { ok = false; break; }
       }
       if (!ok) break;
@@ -450,68 +459,94 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       ++it;
     }
     if (!ok) drain_mma(BAR(drain));
-  } else if (warp >= 4) {
+  } else if (warp < 4) {
+    // base-2 log-sum-exp and delta of the rows, a tile ahead of the compute warps: 64 rows a warp, 16 lanes a row
+    uint32_t it = 0;
+    for (int wave = 0; wave * static_cast<int>(gridDim.x) < items; ++wave) {
+      const int w = snake(wave);
+      if (w >= items) continue;
+      const DqItem t = dq_item(p, w);
+      if (!warp_wait(BAR(stat_empty) + 8 * (it & 1u), ((it >> 1) & 1u) ^ 1u, p.status, ST_TIMEOUT_EMPTY, 404)) break;
+      float* stat = reinterpret_cast<float*>(smem + kDqStat) + (it & 1u) * 256;
+      const int row0 = (warp - 2) * 64;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = row0 + 32 * i + lane;
+        float lse2 = INFINITY;                   // rows past the end, and rows that saw no key, have no probabilities
+        if (t.q0 + row < p.seq) {
+          const float l = p.lse[(static_cast<int64_t>(t.b) * p.q_heads + t.h) * p.seq + t.q0 + row];
+          if (l > -INFINITY) lse2 = l * kLog2e;
+        }
+        stat[row] = lse2;
+      }
+      if (!t.measure) {
+        const size_t at = ((static_cast<size_t>(t.b) * p.seq + t.q0) * p.q_heads + t.h) * kD;
+        const size_t stride = static_cast<size_t>(p.q_heads) * kD;
+        for (int r0 = row0; r0 < row0 + 64; r0 += 16) {
+          uint4 o[8], g[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int row = r0 + 2 * i + (lane >> 4);
+            o[i] = make_uint4(0, 0, 0, 0);
+            g[i] = make_uint4(0, 0, 0, 0);
+            if (t.q0 + row < p.seq) {
+              o[i] = reinterpret_cast<const uint4*>(p.out + at + row * stride)[lane & 15];
+              g[i] = reinterpret_cast<const uint4*>(p.d_out + at + row * stride)[lane & 15];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            Pair sum = mul2(make_pair(bf16_lo(o[i].x), bf16_hi(o[i].x)), make_pair(bf16_lo(g[i].x), bf16_hi(g[i].x)));
+            sum = fma2(make_pair(bf16_lo(o[i].y), bf16_hi(o[i].y)), make_pair(bf16_lo(g[i].y), bf16_hi(g[i].y)), sum);
+            sum = fma2(make_pair(bf16_lo(o[i].z), bf16_hi(o[i].z)), make_pair(bf16_lo(g[i].z), bf16_hi(g[i].z)), sum);
+            sum = fma2(make_pair(bf16_lo(o[i].w), bf16_hi(o[i].w)), make_pair(bf16_lo(g[i].w), bf16_hi(g[i].w)), sum);
+            float lo, hi;
+            split(sum, lo, hi);
+            lo += hi;
+#pragma unroll
+            for (int k = 8; k > 0; k >>= 1) lo += __shfl_xor_sync(kFullMask, lo, k);
+            if ((lane & 15) == 0) stat[kBlk + r0 + 2 * i + (lane >> 4)] = lo;
+          }
+        }
+      }
+      warp_arrive(BAR(stat_full) + 8 * (it & 1u));
+      ++it;
+    }
+  } else {
     const int half = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
     float* red = reinterpret_cast<float*>(smem + kDqRed);
-    uint32_t it = 0, blk = 0;
+    uint32_t it = 0, blk = 0, measured = 0;
     bool ok = true;
-    // a tile's row in O, dO and dQ, and its half of delta and log-sum-exp: fetched for the next tile before this
-    // one's last product has been waited for
-    struct Row { int w; size_t at; float part, lse2; bool live; };
-    auto fetch = [&](int wave) {
-      Row r;
-      r.w = wave * static_cast<int>(gridDim.x) < items ? snake(wave) : items;
-      r.part = 0.0f;
-      r.lse2 = INFINITY;                         // rows past the end, and rows that saw no key, have no probabilities
-      r.live = false;
-      r.at = 0;
-      if (r.w >= items) return r;
-      const DqItem t = dq_item(p, r.w);
-      const int q_pos = t.q0 + row;
-      r.live = q_pos < p.seq;
-      if (!r.live) return r;
-      r.at = ((static_cast<size_t>(t.b) * p.seq + q_pos) * p.q_heads + t.h) * kD + half * 64;
-      const float l = p.lse[(static_cast<int64_t>(t.b) * p.q_heads + t.h) * p.seq + q_pos];
-      if (l > -INFINITY) r.lse2 = l * kLog2e;
-      const uint4* o = reinterpret_cast<const uint4*>(p.out + r.at);
-      const uint4* g = reinterpret_cast<const uint4*>(p.d_out + r.at);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint4 a = o[i], c = g[i];
-        r.part = fmaf(bf16_lo(a.x), bf16_lo(c.x), r.part); r.part = fmaf(bf16_hi(a.x), bf16_hi(c.x), r.part);
-        r.part = fmaf(bf16_lo(a.y), bf16_lo(c.y), r.part); r.part = fmaf(bf16_hi(a.y), bf16_hi(c.y), r.part);
-        r.part = fmaf(bf16_lo(a.z), bf16_lo(c.z), r.part); r.part = fmaf(bf16_hi(a.z), bf16_hi(c.z), r.part);
-        r.part = fmaf(bf16_lo(a.w), bf16_lo(c.w), r.part); r.part = fmaf(bf16_hi(a.w), bf16_hi(c.w), r.part);
-      }
-      return r;
-    };
-    Row next = fetch(0);
     for (int wave = 0; ok && wave * static_cast<int>(gridDim.x) < items; ++wave) {
-      const Row r = next;
-      if (r.w >= items) break;                   // only the last wave is short
-      const DqItem t = dq_item(p, r.w);
+      const int w = snake(wave);
+      if (w >= items) continue;
+      const DqItem t = dq_item(p, w);
       const int q_pos = t.q0 + row;
-      // delta: the two halves of a row's sum exchanged through shared memory, two buffers so that the barrier orders reuse
-      float* red_it = red + (it & 1u) * 256;
-      red_it[half * kBlk + row] = r.part;
-      warp_arrive(BAR(red));
-      if (!warp_wait(BAR(red), it & 1u, p.status, ST_TIMEOUT_FULL, 423)) { ok = false; break; }
-      const float delta = red_it[row] + red_it[kBlk + row];
-      {
-        // for the second kernel: -delta, and the log-sum-exp as it enters S (with a cap: as it is subtracted from y)
-        const int64_t tile = ((static_cast<int64_t>(t.b) * p.q_heads + t.h) * p.seq_pad + t.q0) * 32;
+      const bool live = q_pos < p.seq;
+      float* stat = reinterpret_cast<float*>(smem + kDqStat) + (it & 1u) * 256;
+      if (!warp_wait(BAR(stat_full) + 8 * (it & 1u), (it >> 1) & 1u, p.status, ST_TIMEOUT_FULL, 424)) { ok = false; break; }
+      const float lse2 = stat[row];
+      const Pair minus_lse2 = make_pair(-lse2, -lse2);
+      float delta = t.measure ? 0.0f : stat[kBlk + row];
+      Pair minus_delta = make_pair(-delta, -delta);
+      // for the second kernel: -delta, and the log-sum-exp as it enters S (with a cap: as it is subtracted from y)
+      const int64_t tile = ((static_cast<int64_t>(t.b) * p.q_heads + t.h) * p.seq_pad + t.q0) * 32;
+      auto leave = [&]() {
+        warp_arrive(BAR(stat_empty) + 8 * (it & 1u));
         if (half != 0) store_constant(p.delta + tile, row, -delta);
-        else if (kCap) *reinterpret_cast<float*>(p.lse2 + tile / 8 + row * 4) = -r.lse2;
-        else store_constant(p.lse2 + tile, row, -r.lse2 * p.inv_scale_log2);
-      }
-      const Pair minus_lse2 = make_pair(-r.lse2, -r.lse2), minus_delta = make_pair(-delta, -delta);
-      for (int j = 0; j < t.blocks; ++j, ++blk) {
-        const int key0 = (t.first + j) * kBlk + half * 64;
+        else if (kCap) *reinterpret_cast<float*>(p.lse2 + tile / 8 + row * 4) = -lse2;
+        else store_constant(p.lse2 + tile, row, -lse2 * p.inv_scale_log2);
+      };
+      if (!t.measure) leave();
+      const int from = t.steps - t.blocks;
+      Pair sum = make_pair(0.0f, 0.0f);
+      for (int j = 0; j < t.steps; ++j, ++blk) {
+        const int key0 = (t.first + (j < from ? j : j - from)) * kBlk + half * 64;
         const uint32_t s_addr = t_s + (blk & 1u) * 128 + lane_addr + half * 64;
         if (!warp_wait(BAR(s_full) + 8 * (blk & 1u), (blk >> 1) & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 420)) { ok = false; break; }
         tc_fence_after();
-        const int hi = r.live ? q_pos - key0 + 1 : 0;      // visible keys of this row: [lo, hi) of the 64
+        const int hi = live ? q_pos - key0 + 1 : 0;      // visible keys of this row: [lo, hi) of the 64
         const int lo = p.window > 0 ? q_pos - key0 - p.window + 1 : 0;
         const bool masked = __any_sync(kFullMask, hi < 64 || lo > 0);
         Pair pr[32];
@@ -524,7 +559,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           Pair slope;
           pr[i] = probability<kCap>(i < 16 ? make_pair(v[(2 * i) & 31], v[(2 * i + 1) & 31]) : make_pair(u[(2 * i) & 31], u[(2 * i + 1) & 31]),
                                     minus_lse2, p, slope);
-          if (kCap) pr[i] = mul2(pr[i], slope);
+          if (kCap && j >= from) pr[i] = mul2(pr[i], slope);
         }
         if (!warp_wait(BAR(dp_full), blk & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 421)) { ok = false; break; }
         tc_fence_after();
@@ -533,12 +568,29 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         tc_wait_ld();
         tc_fence_before();
         warp_arrive(BAR(dp_read));
+        auto dp = [&](int i) { return i < 16 ? make_pair(v[(2 * i) & 31], v[(2 * i + 1) & 31]) : make_pair(u[(2 * i) & 31], u[(2 * i + 1) & 31]); };
+        if (j < from) {                            // the first time over: the row's sum of P dP
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sum = add2(sum, keep_range(mul2(pr[i], dp(i)), 2 * i, lo, hi));
+          warp_arrive(BAR(ds_full));
+          if (j == from - 1) {                     // the two halves of the row
+            float a, b;
+            split(sum, a, b);
+            (half == 0 ? stat + kBlk : red)[row] = a + b;
+            warp_arrive(BAR(red));
+            if (!warp_wait(BAR(red), measured & 1u, p.status, ST_TIMEOUT_FULL, 423)) { ok = false; break; }
+            ++measured;
+            delta = stat[kBlk + row] + red[row];
+            minus_delta = make_pair(-delta, -delta);
+            leave();
+          }
+          continue;
+        }
         // one branch per tile: the tests of a masked tile cost as much as the arithmetic
         auto gradients = [&](auto m) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const Pair dp = i < 16 ? make_pair(v[(2 * i) & 31], v[(2 * i + 1) & 31]) : make_pair(u[(2 * i) & 31], u[(2 * i + 1) & 31]);
-            Pair d = mul2(pr[i], add2(dp, minus_delta));
+            Pair d = mul2(pr[i], add2(dp(i), minus_delta));
             if (decltype(m)::value) d = keep_range(d, 2 * i, lo, hi);
             pk[i] = pack_bf16(d);
           }
@@ -551,7 +603,6 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         warp_arrive(BAR(ds_full));
       }
       if (!ok) break;
-      next = fetch(wave + 1);
       if (!warp_wait(BAR(dq_full), it & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 422)) { ok = false; break; }
       tc_fence_after();
       uint32_t a[32], b[32];
