@@ -151,6 +151,11 @@ struct KvWalk {
   }
 };
 
+// The second kernel is launched while the first one ends: its CTAs set up on SMs that are free and wait for the first
+// one's results where they first read them (two sequences of 77: kOverlapNote).
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_first() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // A role's bounded wait; the warp's lanes agree on the outcome. Without a status record a wait that runs out goes
 // unreported, and the CTA's others run out by themselves.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, Status* st, int code, int what) {
@@ -346,6 +351,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     if (threadIdx.x == 0 && p.status != nullptr) report_failure(p.status, ST_BAD_ARGUMENT, 499, sb, 1024);
     return;
   }
+  launch_dependents();
   DqBars* bars = reinterpret_cast<DqBars*>(smem + kDqBar);
   const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 #define BAR(name) PLB_BAR(DqBars, kDqBar, name)
@@ -690,6 +696,7 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       }
       __syncwarp();
       ++it;
+      if (it == 1) wait_for_first();     // K and V are on their way; the queries' constants are the first kernel's
       int g = walk.i0 / t.tiles, qt = walk.i0 % t.tiles;
       for (int i = walk.i0; i < walk.i1; ++i, ++n) {
         const int h = t.h * p.group + g, row = (t.first + qt) * kBlk;
@@ -1042,8 +1049,17 @@ cudaError_t launch_attention_bwd(const AttnBwdArgs& a, cudaStream_t stream) {
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   const int grid = runs.count > 0 ? runs.count : static_cast<int>(kv_items < a.num_sms ? kv_items : a.num_sms);
-  dkdv<<<grid, kBwdThreads, kKvSmem, stream>>>(mq, mdo, mk, mv, p, runs);
-  err = cudaGetLastError();
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(kBwdThreads);
+  config.dynamicSmemBytes = kKvSmem;
+  config.stream = stream;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  err = cudaLaunchKernelEx(&config, dkdv, mq, mdo, mk, mv, p, runs);
   if (err != cudaSuccess || runs.count < 2) return err;
   attention_bwd_join_kernel<<<dim3(runs.count - 1, 8), 256, 0, stream>>>(p, runs);
   return cudaGetLastError();
