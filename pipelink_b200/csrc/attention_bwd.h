@@ -23,7 +23,7 @@ struct AttnBwdParams {
   int64_t seq_pad;           // tiles * 128
   int window;                // 0 = none
   float scale, scale_log2, inv_scale_log2;
-  float cap_in, cap_out;     // soft cap: y = cap_out * tanh in base 2, 2 log2(e) * scale / cap on the way in
+  float cap_in, cap_out;     // soft cap: y = cap_out * tanh(score * cap_in) in base 2
   float4* partial;           // two slots of fp32 sums of dK and dV a run
   Status* status;
 };
