@@ -58,7 +58,7 @@ static_assert(kDqSmem <= 232448 && kKvSmem <= 232448, "227 KB of shared memory p
 
 struct DqBars {
   uint64_t q_full, q_empty, k_full[kDqKStages], k_empty[kDqKStages], v_full[kDqVStages], v_empty[kDqVStages];
-  uint64_t s_full[2], dp_full, dp_read, ds_full, dq_full, dq_free, red, stat_full[2], stat_empty[2], drain;
+  uint64_t s_full[2], dp_full, dp_read, ds_full[2], dq_full, dq_free, red, stat_full[2], stat_empty[2], drain;
   uint32_t tmem_base, pad;
 };
 struct KvBars {
@@ -311,10 +311,6 @@ __device__ __forceinline__ Pair keep_range(Pair p, int i, int lo, int hi) {
   split(p, a, b);
   return make_pair(i >= lo && i < hi ? a : 0.0f, i + 1 >= lo && i + 1 < hi ? b : 0.0f);
 }
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&t);
-}
 // 64 fp32 accumulator columns of each lane's row, scaled, as bf16 to 128 bytes of the row; `rows` of the warp's rows
 // exist, `stride` elements apart from dst on. Eight lanes first exchange their 16-byte chunks so that each store
 // writes whole 128-byte pieces of four rows; a lane storing its own row would touch 32 lines with every store, some
@@ -369,7 +365,9 @@ __device__ __forceinline__ void store_part(const uint32_t (&a)[32], const uint32
 // ------------------------------------------------------------------------------------------ dQ
 // TMEM columns: dQ 0-127, S 128-255 and 256-383 (two buffers), dP 384-511. dX overwrites the S buffer it came
 // from, as the A operand of dQ += dX K. dP(j+1) is issued as soon as dP(j) has been read into registers, S(j+2) as
-// soon as dQ(j) has released its buffer, so the compute warps find their next operands ready.
+// soon as dQ(j) has released its buffer, so the compute warps find their next operands ready. A warp that is done with
+// dX(j) may therefore finish dX(j+1) before another is done with dX(j) (a warp without masked pairs before one with some):
+// consecutive blocks report on two barriers, or its second arrival would count for the other warp's first.
 template <bool kCap>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
@@ -395,6 +393,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     mbar_init(BAR(dp_full), 1);
     mbar_init(BAR(dp_read), kComputeWarps);
     mbar_init(BAR(ds_full), kComputeWarps);
+    mbar_init(BAR(ds_full) + 8, kComputeWarps);
     mbar_init(BAR(dq_full), 1);
     mbar_init(BAR(dq_free), kComputeWarps);
     mbar_init(BAR(red), kComputeWarps);
@@ -482,7 +481,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         if (!warp_wait(BAR(dp_read), blk & 1u, p.status, ST_TIMEOUT_FULL, 415)) { ok = false; break; }
         if (j + 1 < n && !issue_dp(blk + 1)) { ok = false; break; }
         if (j + 2 == n) warp_commit(BAR(q_empty));       // the last products that read Q and dO are issued: both may be replaced
-        if (!warp_wait(BAR(ds_full), blk & 1u, p.status, ST_TIMEOUT_FULL, 413)) { ok = false; break; }
+        if (!warp_wait(BAR(ds_full) + 8 * (blk & 1u), (blk >> 1) & 1u, p.status, ST_TIMEOUT_FULL, 413)) { ok = false; break; }
         if (j == from && !warp_wait(BAR(dq_free), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_TMEM_EMPTY, 414)) { ok = false; break; }
         tc_fence_after();
         const uint32_t ks = blk % kDqKStages;
@@ -612,7 +611,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         if (j < from) {                            // the first time over: the row's sum of P dP
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum = add2(sum, keep_range(mul2(pr[i], dp(i)), 2 * i, lo, hi));
-          warp_arrive(BAR(ds_full));
+          warp_arrive(BAR(ds_full) + 8 * (blk & 1u));
           if (j == from - 1) {                     // the two halves of the row
             float a, b;
             split(sum, a, b);
@@ -640,7 +639,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         tc_st_32x32b_x32(s_addr, pk);
         tc_wait_st();
         tc_fence_before();
-        warp_arrive(BAR(ds_full));
+        warp_arrive(BAR(ds_full) + 8 * (blk & 1u));
       }
       if (!ok) break;
       if (!warp_wait(BAR(dq_full), it & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 422)) { ok = false; break; }

@@ -93,6 +93,20 @@ def test_gradients_against_the_formula(native_lib, B, S, Hq, Hkv, window, softca
     check(att.attention_bwd(do, q, k, v, out, lse, window=window, softcap=softcap), grads, tol)
 
 
+@pytest.mark.parametrize("S,window", [(900, 300), (385, 0), (200, 0)])
+def test_same_bits_in_every_call(native_lib, S, window):
+    """Warps of a tile with and without masked pairs take different times; the gradients do not depend on it. Copies of the
+    inputs change the times of the first loads."""
+    from pipelink_b200 import attention as att
+    q, k, v, do = make(1, S, 4, 2, seed=S)
+    out, lse, _, _ = reference(q, k, v, do, window)
+    first = att.attention_bwd(do, q, k, v, out, lse, window=window)
+    for i in range(600):
+        args = [t.clone() for t in (do, q, k, v, out, lse)]
+        got = att.attention_bwd(*args, window=window, check=i % 2 == 0)
+        assert all(torch.equal(a, b) for a, b in zip(got, first)), i
+
+
 def test_large_scores(native_lib):
     """Probabilities from 1 down to underflow, and masked scores far above the row's log-sum-exp."""
     from pipelink_b200 import attention as att
