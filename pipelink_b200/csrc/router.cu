@@ -5,13 +5,14 @@
 //   the topk best c of the kept groups, ties to the lowest index; w = scale * s [/ sum of the chosen s]
 //   dS_j = scale / S * (g_j - sum_i g_i s_i / S) or scale * g_j;  dx = s (dS - sum s dS) or dS s (1 - s)
 //
-// One warp per token, NV consecutive experts to a lane. The topk-th largest of the 32 lanes' maxima bounds
-// the topk-th value from below: what is not under it, some 10 to 20 candidates, is put one to a lane and ranked by
-// comparing each with each (16384 tokens, 256 experts, 8 chosen: 19 us, with rounds of maxima 26). Where that leaves more than 32 (many
-// ties, a large topk), topk rounds of a warp-wide maximum choose. Without a bias the scores are ordered as the logits are, and those are compared as they
-// stand. With one (or with sums of two scores over groups) the order is that of numbers fp32 may not tell apart.
-// Every comparison that matters is checked against the bound of the fp32 scores' error; candidates closer than that
-// are put in order by their fp64 values (some 2 tokens of 1000 at 256 experts).
+// One warp per token, NV consecutive experts to a lane. The topk-th largest of the 32 lanes' maxima bounds the topk-th
+// value from below: what is not under it, some 10 to 20 candidates, is put one to a lane and ranked by comparing each
+// with each (16384 tokens, 256 experts, 8 chosen: 13 us; with rounds of maxima it was 7 us more). Where that leaves
+// more than 32 (many ties, a large topk), topk rounds of a warp-wide maximum choose. Without a bias the scores are
+// ordered as the logits are, and those are compared as they stand. With one (or with sums of two scores over groups) the
+// order is that of numbers fp32 may not tell apart. Every comparison that matters is checked against the bound of the
+// fp32 scores' error; candidates closer than that are put in order by their fp64 values (some 2 tokens of 1000 at 256
+// experts).
 #include <math.h>
 
 #include <type_traits>
@@ -247,8 +248,9 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
   auto score = [&](float x) { return a.sigmoid ? __fdividef(1.0f, 1.0f + expf(-x)) : expf(x - top) * inv_sum; };
   // How far two fp32 choice values must lie apart to be in the order of the exact ones: twice the error of a score,
   // and the roundings of the sums (under 2^-23 of |c| + 1/4 each). A sigmoid is off by the two steps of expf (2^-23
-  // each), the sum's half step and the quotient's two: 2^-20.8 at most. A softmax by two steps of expf, the sum's NV + 5 roundings, six
-  // more, and half a step of |x - top|, which is largest against exp(top - x) at 1: under (NV + 16) 2^-23 of the largest.
+  // each), the sum's half step and the quotient's two: 2^-20.8 at most. A softmax by two steps of expf, the sum's NV + 5
+  // roundings, six more, and half a step of |x - top|, which is largest against exp(top - x) at 1: under (NV + 16) 2^-23
+  // of the largest.
   const float slack = a.sigmoid ? 1.1e-6f : (NV + 16) * 2.4e-7f * inv_sum;
   auto near = [&](float high, float low) { return high - low <= slack + 2.4e-7f * (fabsf(high) + 0.25f); };   // NaN and inf - inf: not near
   if (by_score || by_sum) {
@@ -449,8 +451,13 @@ route_topk_bwd_kernel(const __grid_constant__ RouteBwdArgs a) {
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    s[i] = a.sigmoid ? 1.0f / (1.0f + expf(-s[i])) : expf(s[i] - top);
-    if (!a.sigmoid) sum += s[i];
+    if (a.sigmoid) {               // the slope s (1 - s), without the difference that cancels where s is near 1
+      const float e = expf(-fabsf(s[i]));
+      s[i] = e / ((1.0f + e) * (1.0f + e));
+    } else {
+      s[i] = expf(s[i] - top);
+      sum += s[i];
+    }
   }
   if (!a.sigmoid) {
     sum = warp_sum(sum);
@@ -491,7 +498,7 @@ route_topk_bwd_kernel(const __grid_constant__ RouteBwdArgs a) {
   }
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < NV; ++i) s[i] = a.sigmoid ? ds[e0 + i] * s[i] * (1.0f - s[i]) : s[i] * (ds[e0 + i] - dot);
+  for (int i = 0; i < NV; ++i) s[i] = a.sigmoid ? ds[e0 + i] * s[i] : s[i] * (ds[e0 + i] - dot);
   if (e0 >= a.experts) return;
   const int64_t out = token * a.experts + e0;
   if (a.bf16) {

@@ -180,6 +180,17 @@ def test_gradient(native_lib, tokens, experts, k, score, renormalize):
         assert got.dtype == dtype and ((got.double() - want).abs() <= tol).all(), float(((got.double() - want).abs() / tol).max())
 
 
+def test_gradient_of_saturated_sigmoids(native_lib):
+    """Far from 0 the slope s (1 - s) is small but as exact as anywhere: expf is off by two steps, the rest by one each."""
+    from pipelink_b200 import router
+    x = torch.linspace(-40, 40, 32, device="cuda")[None].contiguous()
+    chosen = torch.arange(32, dtype=torch.int32, device="cuda")[None]
+    dw = 1 + torch.rand(1, 32, device="cuda")
+    got = router.route_topk_bwd(dw, x, chosen, score="sigmoid", renormalize=False)
+    want = dw.double() * torch.sigmoid(x.double()) * torch.sigmoid(-x.double())
+    assert ((got.double() - want).abs() <= 16 * F * want).all()
+
+
 def test_gradient_of_masked_repeated_and_foreign_experts(native_lib):
     from pipelink_b200 import router
     x = torch.randn(4, 40, device="cuda")
