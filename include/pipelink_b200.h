@@ -546,7 +546,7 @@ int plb_tp_gemm_bf16(const void* a_bf16, const void* b_bf16, const int32_t* bloc
  * neither read as keys nor written). The probabilities are recomputed from lse; dk and dv are summed over the
  * query heads of their group in fp32 and rounded once, with no atomics: the same inputs give the same bits.
  * workspace: plb_attention_bwd_workspace_bytes() bytes, written and read by this call alone (its contents before and
- * after mean nothing). status may be NULL: a bounded wait that runs out then goes unreported. Rows must be finite:
+ * after mean nothing). scale and softcap are finite, scale positive. status may be NULL: a bounded wait that runs out then goes unreported. Rows must be finite:
  * a masked pair's probability is 0, and 0 times an infinity of the pair's other operand is NaN. The reference has
  * no backward pass of its attention campaign. */
 size_t plb_attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv_heads, int window);
@@ -565,6 +565,7 @@ int plb_attention_bwd(const void* q, const void* k, const void* v, const void* o
  * plb_rmsnorm_bwd: d_x = rstd * (g - n * mean(g * n)) + d_hidden with g = d_y * weight, n = hidden * rstd (the
  * gradient of x and of residual alike; d_hidden, the gradient that reaches hidden past the norm, may be NULL);
  * d_weight f32 [width] = sum over rows of d_y * n, in a fixed order. hidden is what the forward pass normalised.
+ * workspace: plb_rmsnorm_bwd_workspace_bytes() bytes, 16-byte aligned; d_x overlaps no input.
  * The reference normalises inside its decode megakernel only (campaigns/megakernel/host/mk_host_abi.h:35-85). */
 int plb_rmsnorm_fwd(const void* x, int64_t ld_x, const void* residual, int64_t ld_residual, const void* weight, int64_t rows,
                     int64_t width, float eps, void* hidden, float* rstd, void* y, void* fp8, void* sc, void* stream);

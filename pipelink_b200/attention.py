@@ -124,7 +124,7 @@ def attention_bwd(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
     for t in (d_out, q, k, v, out):
         if t.dtype is not torch.bfloat16 or t.device != dev or dev.type != "cuda":
             raise ValueError("attention_bwd wants bf16 CUDA tensors on one device")
-    if window < 0 or not softcap >= 0.0:
+    if window < 0 or not 0.0 <= softcap < math.inf:
         raise ValueError("window and softcap are 0 (off) or positive")
     with device_of(q):
         d_out, q, k, v, out, lse = dense(d_out), dense(q), dense(k), dense(v), dense(out), dense(lse)

@@ -2,7 +2,10 @@
 // Declarations and their reference counterparts are in include/pipelink_b200.h.
 #include "../../include/pipelink_b200.h"
 
+#include <float.h>
 #include <string.h>
+
+#include <atomic>
 
 #include "attention.h"
 #include "attention_bwd.h"
@@ -32,9 +35,12 @@ int from_cuda(cudaError_t err) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int sm_count() {
+  static std::atomic<int> known[64];       // per device, 0 = not asked yet
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 64 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
   return sms;
 }
 
@@ -1029,7 +1035,8 @@ size_t plb_attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv
 int plb_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* d_out, const float* lse,
                       void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, int batch, int seq, int q_heads,
                       int kv_heads, float scale, int window, float softcap, plb_status* status, void* stream) {
-  if (!attention_bwd_shape_ok(batch, seq, q_heads, kv_heads, window) || !(softcap >= 0.0f) || !(scale > 0.0f)) return PLB_E_ARGUMENT;
+  if (!attention_bwd_shape_ok(batch, seq, q_heads, kv_heads, window) || !(scale >= FLT_MIN && scale <= FLT_MAX)) return PLB_E_ARGUMENT;
+  if (!(softcap >= 0.0f && softcap <= FLT_MAX) || (softcap > 0.0f && scale / softcap > FLT_MAX)) return PLB_E_ARGUMENT;
   if (batch == 0 || seq == 0) return PLB_OK;
   if (!q || !k || !v || !out || !d_out || !lse || !dq || !dk || !dv || !workspace) return PLB_E_ARGUMENT;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(d_out) || !aligned16(dq) ||

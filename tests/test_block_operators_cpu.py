@@ -18,7 +18,7 @@ def test_attention_bwd_refusals(native_lib):
     assert need(2, 129, 3, 1, 0) >= 2 * 2 * 3 * 256 * 4 and need(1, 8192, 32, 8, 0) >= 2 * 32 * 8192 * 4
     assert need(0, 129, 3, 1, 0) == 0 and need(2, 129, 3, 2, 0) == 0 and need(1, 128, 1, 1, -1) == 0
     for bad in (dict(batch=-1), dict(seq=-1), dict(q_heads=0), dict(kv_heads=0), dict(q_heads=5), dict(window=-1), dict(softcap=-1.0),
-                dict(softcap=float("nan")), dict(ptr=None), dict(ptr=4104), dict(last=None), dict(seq=2 ** 30 + 1), dict(batch=2 ** 23, seq=2 ** 20)):
+                dict(softcap=float("nan")), dict(softcap=float("inf")), dict(softcap=1e-40), dict(ptr=None), dict(ptr=4104), dict(last=None), dict(seq=2 ** 30 + 1), dict(batch=2 ** 23, seq=2 ** 20)):
         assert bwd(native_lib, **bad) in (ARGUMENT, CAPACITY), bad
     assert bwd(native_lib, nbytes=100) == CAPACITY
     assert bwd(native_lib, batch=0) == OK and bwd(native_lib, seq=0) == OK
