@@ -217,6 +217,7 @@ class MoKHost:
             bf = dict(dtype=torch.bfloat16, device=self.device)
             self.buffers.update(x_routed_bf16=torch.empty((P, H), **bf), hidden_routed_bf16=torch.empty((P, I), **bf))
         self.weights = None
+        self.block = None      # load_block
 
     # ------------------------------------------------------------------ weights
     def load_weights(self, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
@@ -553,6 +554,8 @@ class MoKHost:
         if self.weights is None:
             raise RuntimeError("load_weights() first")
         self.status.reset()
+        if self.block is not None:
+            self.block["kept"] = None       # backward_block would mix the two calls
         self.schedule_into(inputs.experts[None])
         self.x_buffer.copy_(inputs.x)
         self.router_weight_buffer.copy_(inputs.router)
@@ -586,7 +589,7 @@ class MoKHost:
                           gate=gate_weight.to(dtype=torch.bfloat16, **on).contiguous(),
                           bias=None if gate_bias is None else gate_bias.to(dtype=torch.float32, **on).contiguous(),
                           hidden=torch.empty((sh.tokens, sh.hidden), dtype=torch.bfloat16, **on),
-                          rstd=torch.empty(sh.tokens, dtype=torch.float32, **on))
+                          rstd=torch.empty(sh.tokens, dtype=torch.float32, **on), kept=None)
 
     def forward_block(self, x: torch.Tensor, residual: torch.Tensor | None = None, *, check: bool = True, train: bool = False):
         """The expert branch of a transformer block (single rank): hidden = x + residual, its RMS norm, the router, the
@@ -596,17 +599,19 @@ class MoKHost:
         from . import norm, router
         if self.world != 1:
             raise ValueError("forward_block() drives one rank")
-        if getattr(self, "block", None) is None or self.weights is None:
+        if self.block is None or self.weights is None:
             raise RuntimeError("load_weights() and load_block() first")
         if train and "w_down_t_fp8" not in self.weights and "w_down_t_bf16" not in self.weights:
             raise RuntimeError("load_weights(..., train=True) first")
         blk, mx = self.block, self.precision == "mxfp8"
-        if tuple(x.shape) != (self.shape.tokens, self.shape.hidden):
-            raise ValueError("x disagrees with the session shape")
+        if x.shape != blk["hidden"].shape or x.dtype is not torch.bfloat16 or x.device != blk["hidden"].device:
+            raise ValueError("x is bf16 [tokens, hidden] on the session's device")
         self.status.reset()
-        n = norm.rmsnorm_fwd(x, blk["norm"], residual, eps=blk["eps"], out="both" if mx else "bf16",
-                             into=norm.Normed(blk["hidden"], blk["rstd"], self.x_buffer, self.xq if mx else None, self.xsc if mx else None))
-        blk["stream"] = n.hidden if residual is not None else x
+        blk["kept"] = None
+        if residual is None:                # the session keeps the stream: x may be its own output, written again below
+            x = blk["hidden"].copy_(x)
+        norm.rmsnorm_fwd(x, blk["norm"], residual, eps=blk["eps"], out="both" if mx else "bf16",
+                         into=norm.Normed(blk["hidden"], blk["rstd"], self.x_buffer, self.xq if mx else None, self.xsc if mx else None))
         if mx:
             self.token_scale_rows()
         blk["logits"] = torch.mm(self.x_buffer, blk["gate"].T, out_dtype=torch.float32)
@@ -620,9 +625,10 @@ class MoKHost:
             self.gemm_gate_up()
         self.gemm_down()
         out = self.fwd_epilogue()
+        blk["kept"] = "train" if train else "recompute"
         if check:
             self.status.check("after a block's forward pass")
-        return {"output": out, "hidden": blk["stream"], "experts": self.routes_i32[0], "router": self.router_weight_buffer,
+        return {"output": out, "hidden": blk["hidden"], "experts": self.routes_i32[0], "router": self.router_weight_buffer,
                 "logits": blk["logits"], **self.context_tensors()}
 
     def backward_block(self, d_out: torch.Tensor, d_hidden: torch.Tensor | None = None, *, check: bool = True, recompute: bool = False):
@@ -630,14 +636,18 @@ class MoKHost:
         "output", `d_hidden` what reaches "hidden" from behind. Returns d_x (of x and of the residual alike), d_norm_weight,
         d_gate_weight (f32) and the experts' gradients as ``backward`` names them."""
         from . import norm, router
-        blk = getattr(self, "block", None)
-        if blk is None or "logits" not in blk:
+        blk = self.block
+        if blk is None or blk["kept"] is None:
             raise RuntimeError("forward_block() first")
-        g = self.backward(d_out, check=False, recompute=recompute)
+        if blk["kept"] == "recompute" and not recompute:
+            raise RuntimeError("forward_block(train=True) first, or recompute=True")
+        if d_out.shape != blk["hidden"].shape or d_out.dtype is not torch.bfloat16 or d_out.device != blk["hidden"].device:
+            raise ValueError("d_out is bf16 [tokens, hidden] on the session's device")
+        g = self.backward(dense(d_out), check=False, recompute=recompute)
         routing = {k: v for k, v in blk["routing"].items() if k in ("score", "renormalize", "scale")}
         d_logits = router.route_topk_bwd(g["d_router_weights"], blk["logits"], self.routes_i32[0], **routing)
         d_y = torch.addmm(g["d_x"].float(), d_logits, blk["gate"].float()).to(torch.bfloat16)
-        d_x, d_norm = norm.rmsnorm_bwd(d_y, blk["stream"], blk["rstd"], blk["norm"], d_hidden)
+        d_x, d_norm = norm.rmsnorm_bwd(d_y, blk["hidden"], blk["rstd"], blk["norm"], d_hidden)
         if check:
             self.status.check("after a block's backward pass")
         return {**g, "d_x": d_x, "d_norm_weight": d_norm, "d_gate_weight": d_logits.T @ self.x_buffer.float()}

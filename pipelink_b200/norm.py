@@ -74,7 +74,7 @@ def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
         _lib.call("plb_rmsnorm_fwd", x2.data_ptr(), ld_x, _ptr(r2), ld_r, weight.data_ptr(), rows, width, eps,
                   into.hidden.data_ptr() if residual is not None else 0, into.rstd.data_ptr(), _ptr(into.y), _ptr(into.fp8),
                   _ptr(into.sc), _stream())
-    return into
+    return into if residual is not None else into._replace(hidden=x)
 
 
 def rmsnorm_bwd(d_y: torch.Tensor, hidden: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor,

@@ -132,3 +132,34 @@ def test_branch_refusals(native_lib):
     with pytest.raises(ValueError):
         host.forward_block(x[:32])
     assert (host.forward_block(x)["output"] == 0).all()
+
+
+def test_branch_of_its_own_output(native_lib):
+    """x may be the tensor an earlier call returned, and its gradients are still those of the values it had."""
+    host, w, x, _, d_out = session(("own", 4, 256, 256, 2, 200), "bf16", train=True, seed=5)
+    first = host.forward_block(x, train=True)["output"]
+    kept = first.clone()
+    host.forward_block(first, train=True)
+    got = {k: v.clone() for k, v in host.backward_block(d_out.T.contiguous().T).items()}     # strides other than the tested
+    host.forward_block(kept, train=True)
+    for name, value in host.backward_block(d_out).items():
+        assert torch.equal(value, got[name]), name
+
+
+def test_branch_order_of_calls(native_lib):
+    from pipelink_b200 import mok
+    host, _, x, _, d_out = session(("order", 4, 256, 256, 1, 128), "bf16", train=True)
+    got = host.forward_block(x)
+    with pytest.raises(RuntimeError):                 # kept nothing for the backward pass
+        host.backward_block(d_out)
+    with pytest.raises(ValueError):
+        host.backward_block(d_out[:64], recompute=True)
+    with pytest.raises(ValueError):
+        host.backward_block(d_out.float(), recompute=True)
+    with pytest.raises(ValueError):
+        host.forward_block(x.float())
+    host.forward_block(x)
+    host.backward_block(d_out, recompute=True)
+    host.forward(mok.Inputs(x, got["experts"].clone(), got["router"].clone()), train=True)
+    with pytest.raises(RuntimeError):                 # another call's routes and rows are in the buffers
+        host.backward_block(d_out)

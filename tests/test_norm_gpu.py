@@ -113,6 +113,15 @@ def test_strides_alignment_broadcast_and_shapes(native_lib):
     assert torch.equal(stream, want.hidden) and torch.equal(into.y, want.y)
 
 
+def test_reused_outputs(native_lib):
+    """`into` of an earlier call: the result names this call's stream."""
+    from pipelink_b200 import norm
+    x, r, w, _ = make(9, 256, seed=11)
+    first = norm.rmsnorm_fwd(x, w)
+    n = norm.rmsnorm_fwd(r, w, into=first)
+    assert n.hidden is r and n.y is first.y and torch.equal(n.y, norm.rmsnorm_fwd(r, w).y)
+
+
 def test_extremes(native_lib):
     """Rows of zeros, of the largest and the smallest numbers, and rows that hold infinities or NaN."""
     from pipelink_b200 import norm
