@@ -65,6 +65,11 @@ def dense(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def like(t: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of the same shape and type (empty_like keeps strides; new_empty takes twice its host time)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def rows_of(t: torch.Tensor):
     """[..., width] as rows of unit-stride elements and their stride: a view where one exists (a slice of a wider
     tensor, a broadcast row), a copy otherwise."""

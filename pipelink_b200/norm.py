@@ -11,7 +11,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .mok import _ptr, _stream, dense, device_of, rows_of
+from .mok import _ptr, _stream, dense, device_of, like, rows_of
 
 
 class Normed(NamedTuple):
@@ -64,11 +64,12 @@ def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
         r2, ld_r = rows_of(residual) if residual is not None else (None, 0)
         weight = dense(weight)
         if into is None:
-            into = Normed(x.new_empty(shape) if residual is not None else x,
-                          x.new_empty(rows, dtype=torch.float32),
-                          x.new_empty(shape) if out != "mxfp8" else None,
-                          x.new_empty((padded, width), dtype=torch.uint8) if out != "bf16" else None,
-                          x.new_empty((padded // 128, width // 128, 32, 16), dtype=torch.uint8) if out != "bf16" else None)
+            fp8 = sc = None
+            if out != "bf16":
+                fp8 = x.new_empty((padded, width), dtype=torch.uint8)
+                sc = x.new_empty((padded // 128, width // 128, 32, 16), dtype=torch.uint8)
+            into = Normed(like(x) if residual is not None else x, x.new_empty(rows, dtype=torch.float32),
+                          like(x) if out != "mxfp8" else None, fp8, sc)
         else:
             _check_into(into, residual, out, rows, width, padded, dev)
         _lib.call("plb_rmsnorm_fwd", x2.data_ptr(), ld_x, _ptr(r2), ld_r, weight.data_ptr(), rows, width, eps,
@@ -99,7 +100,7 @@ def rmsnorm_bwd(d_y: torch.Tensor, hidden: torch.Tensor, rstd: torch.Tensor, wei
         h2, ld_h = rows_of(hidden)
         e2, ld_e = rows_of(d_hidden) if d_hidden is not None else (None, 0)
         rstd, weight = rstd.contiguous(), dense(weight)
-        d_x = hidden.new_empty(shape)
+        d_x = like(hidden)
         d_weight = hidden.new_empty(width, dtype=torch.float32)
         nbytes = _lib.load().plb_rmsnorm_bwd_workspace_bytes(rows, width)
         workspace = hidden.new_empty(nbytes, dtype=torch.uint8)

@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .mok import _ptr, _stream, device_of, rows_of
+from .mok import _ptr, _stream, device_of, like, rows_of
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _DTYPES = (torch.float32, torch.bfloat16)
@@ -79,7 +79,7 @@ def route_topk_bwd(d_weights: torch.Tensor, logits: torch.Tensor, experts: torch
     with device_of(logits):
         x, ld = rows_of(logits)
         d_weights, experts = d_weights.contiguous(), experts.contiguous()
-        d_logits = logits.new_empty(logits.shape)
+        d_logits = like(logits)
         _lib.call("plb_route_topk_bwd", d_weights.data_ptr(), x.data_ptr(), ld, int(x.dtype == torch.bfloat16), experts.data_ptr(),
                   tokens, logits.shape[1], topk, _SCORES[score], int(renormalize), float(scale), d_logits.data_ptr(), _stream())
     return d_logits
