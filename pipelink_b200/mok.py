@@ -51,12 +51,15 @@ def _ptr(t):
 
 def _stream():
     # the handle of torch.cuda.current_stream(), without the Stream object around it (a tenth of its host time)
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+_HERE = contextlib.nullcontext()
 
 
 def device_of(t: torch.Tensor):
     """Context in which launches go to the tensor's device (its current stream there)."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def dense(t: torch.Tensor) -> torch.Tensor:

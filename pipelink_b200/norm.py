@@ -22,9 +22,18 @@ class Normed(NamedTuple):
     sc: torch.Tensor | None     # u8 [that / 128, width / 128, 32, 16]
 
 
-def _check(name, t, device, shape):
-    if t.dtype is not torch.bfloat16 or t.device != device or t.shape != shape or device.type != "cuda":
-        raise ValueError(f"{name} is a bf16 tensor of shape {tuple(shape)} on one CUDA device")
+def _check(weight, *rows):
+    """Width and device of the rows, which have one shape [..., width] (None: one that is not given)."""
+    shape, device = rows[0].shape, rows[0].device
+    width = shape[-1] if shape else 0
+    if width < 1:
+        raise ValueError("rows are [..., width]")
+    for t in rows:
+        if t is not None and (t.dtype is not torch.bfloat16 or t.shape != shape or t.device != device or not t.is_cuda):
+            raise ValueError(f"the rows are bf16 tensors of one shape, here {tuple(shape)}, on one CUDA device")
+    if weight.dtype is not torch.bfloat16 or weight.shape != (width,) or weight.device != device:
+        raise ValueError(f"weight is bf16 [{width}] on the rows' device")
+    return width, device
 
 
 def _check_into(into: Normed, residual, out, rows, width, padded, device):
@@ -45,14 +54,7 @@ def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
     an earlier call of the same shape, or a session's buffers) instead of new ones; its hidden may be the residual itself."""
     if out not in ("bf16", "mxfp8", "both"):
         raise ValueError("out is 'bf16', 'mxfp8' or 'both'")
-    shape, dev = x.shape, x.device
-    width = shape[-1] if shape else 0
-    if width < 1:
-        raise ValueError("x is [..., width]")
-    _check("x", x, dev, shape)
-    _check("weight", weight, dev, (width,))
-    if residual is not None:
-        _check("residual", residual, dev, shape)
+    width, dev = _check(weight, x, residual)
     if not eps >= 0.0:
         raise ValueError("eps is not negative")
     if out != "bf16" and width % 128:
@@ -83,16 +85,8 @@ def rmsnorm_bwd(d_y: torch.Tensor, hidden: torch.Tensor, rstd: torch.Tensor, wei
     """Gradient of ``rmsnorm_fwd``: (d_x, d_weight). d_x (bf16, like hidden) is the gradient of x and of the residual alike,
     d_weight f32 [width]. `d_hidden` is the gradient that reaches the residual stream past the norm. An MXFP8 output has
     its bf16 value's gradient. The same inputs give the same bits."""
-    shape, dev = hidden.shape, hidden.device
-    width = shape[-1] if shape else 0
-    if width < 1:
-        raise ValueError("hidden is [..., width]")
+    width, dev = _check(weight, hidden, d_y, d_hidden)
     rows = hidden.numel() // width
-    _check("hidden", hidden, dev, shape)
-    _check("d_y", d_y, dev, shape)
-    _check("weight", weight, dev, (width,))
-    if d_hidden is not None:
-        _check("d_hidden", d_hidden, dev, shape)
     if rstd.shape != (rows,) or rstd.dtype is not torch.float32 or rstd.device != dev:
         raise ValueError("rstd is f32 [rows], as rmsnorm_fwd returns it")
     with device_of(hidden):
