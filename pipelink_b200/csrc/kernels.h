@@ -204,7 +204,7 @@ struct RouteArgs {
   int experts, topk, groups, topk_groups;
   int group_share;           // lanes that look through a group: the largest power of two with group_share * groups <= 32
   bool bf16, sigmoid, group_top2, renormalize;
-  bool wide;                 // set by the launcher: lanes load whole pieces of a row
+  bool wide, wide_bias;      // set by the launcher: lanes load whole pieces of a row, of the bias
   float scale;
   int* experts_out;          // [tokens, topk]
   float* weights_out;

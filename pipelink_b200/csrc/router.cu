@@ -7,7 +7,7 @@
 //
 // One warp per token, NV consecutive experts to a lane. The topk-th largest of the 32 lanes' maxima bounds the topk-th
 // value from below: what is not under it, some 10 to 20 candidates, is put one to a lane and ranked by comparing each
-// with each (16384 tokens, 256 experts, 8 chosen: 13 us; with rounds of maxima it was 7 us more). Where that leaves
+// with each (16384 tokens, 256 experts, 8 chosen: 11.4 us; rounds of maxima took 7 us more). Where that leaves
 // more than 32 (many ties, a large topk), topk rounds of a warp-wide maximum choose. Without a bias the scores are
 // ordered as the logits are, and those are compared as they stand. With one (or with sums of two scores over groups) the
 // order is that of numbers fp32 may not tell apart. Every comparison that matters is checked against the bound of the
@@ -71,6 +71,12 @@ __device__ __forceinline__ void load_logits(const void* p, int64_t row, int expe
     }
   }
 }
+// Sigmoid for a choice, whose error the comparisons allow for (see slack); weights are computed with expf.
+__device__ __forceinline__ float choice_sigmoid(float x) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+  return __fdividef(1.0f, 1.0f + e);
+}
 // Unsigned integers in the order of the numbers; NaN below every number, 0 is left for "not a candidate".
 __device__ __forceinline__ uint64_t order_key(double v) {
   if (v != v) return 1;
@@ -81,7 +87,6 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t b = __float_as_uint(v + 0.0f);            // -0 becomes 0
   return v != v ? 1u : b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
-constexpr uint32_t kMasked = 0x007FFFFFu;                   // the key of -inf
 __device__ __forceinline__ float key_value(uint32_t k) {   // the number of a key that is one
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
@@ -209,10 +214,14 @@ __device__ __noinline__ int exact_choice(const RouteArgs& a, int64_t token, uint
   return pick;
 }
 
+// kScored: the choice needs the scores, for a bias or the sums of two; without them no comparison is ever close, and the
+// kernel has neither the tests nor the fp64 paths (65536 x 128: 33 us with them, 28 without).
+//
 // CTAs per SM: what hides the latencies of a token's steps is other tokens, at the price of registers where a lane
-// holds few experts (256 experts in groups: 32 us with 24 warps an SM, 27 with 48).
-template <int NV>
-__global__ void __launch_bounds__(kRouteWarps * 32, NV <= 8 ? 12 : NV <= 16 ? 8 : 4)
+// holds few experts (256 experts in groups with a bias: 18.1 us with 40 warps an SM, 18.5 with 48; by logits alone 48 are
+// as good or better).
+template <int NV, bool kScored>
+__global__ void __launch_bounds__(kRouteWarps * 32, NV <= 8 ? (kScored ? 10 : 12) : NV <= 16 ? 8 : 4)
 route_topk_kernel(const __grid_constant__ RouteArgs a) {
   extern __shared__ __align__(16) uint64_t shared[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -224,13 +233,13 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
   uint32_t key[NV];
   float top = -INFINITY;
   load_logits<NV>(a.logits, token * a.ld_logits, a.experts, a.bf16, a.wide, c);
+  const bool by_score = kScored && a.bias != nullptr;             // else by logits
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    key[i] = e0 + i < a.experts ? order_key(c[i]) : 0;
+    key[i] = !by_score && e0 + i < a.experts ? order_key(c[i]) : 0;
     top = fmaxf(top, c[i]);
   }
-  const bool by_score = a.bias != nullptr;                        // else by logits
-  const bool by_sum = a.groups > 1 && a.group_top2;
+  const bool by_sum = kScored && a.groups > 1 && a.group_top2;
   float inv_sum = 1.0f;
   if (!a.sigmoid) {
     top = warp_max(top);
@@ -240,26 +249,31 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
     for (int i = 0; i < NV; ++i) {
       const float e = expf(c[i] - top);
       sum += e;
-      if (by_score || by_sum) c[i] = e;
+      if (by_score || by_sum) c[i] = c[i] == -INFINITY ? -1.0f : e;      // a masked one stays known
     }
     sum = warp_sum(sum);
     inv_sum = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
   }
   auto score = [&](float x) { return a.sigmoid ? __fdividef(1.0f, 1.0f + expf(-x)) : expf(x - top) * inv_sum; };
   // How far two fp32 choice values must lie apart to be in the order of the exact ones: twice the error of a score,
-  // and the roundings of the sums (under 2^-23 of |c| + 1/4 each). A sigmoid is off by the two steps of expf (2^-23
-  // each), the sum's half step and the quotient's two: 2^-20.8 at most. A softmax by two steps of expf, the sum's NV + 5
+  // and the roundings of the sums (under 2^-23 of |c| + 1/4 each). A sigmoid is off by s (1 - s) times e's relative error
+  // (2^-22 of exp2, and under 2^-23.7 |x| of its argument's roundings), by the sum's half step and the quotient's two steps:
+  // with s (1 - s) at most 1/4, and |x| s (1 - s) 0.224, 2^-24 + 2^-25.8 + 2^-24 + 2^-22, twice that under 2^-20.3. A softmax by two steps of expf, the sum's NV + 5
   // roundings, six more, and half a step of |x - top|, which is largest against exp(top - x) at 1: under (NV + 16) 2^-23
   // of the largest.
   const float slack = a.sigmoid ? 1.1e-6f : (NV + 16) * 2.4e-7f * inv_sum;
   auto near = [&](float high, float low) { return high - low <= slack + 2.4e-7f * (fabsf(high) + 0.25f); };   // NaN and inf - inf: not near
   if (by_score || by_sum) {
+    float bias[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) bias[i] = 0.0f;
+    if (by_score) load_logits<NV>(a.bias, 0, a.experts, false, a.wide_bias, bias);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (e0 + i >= a.experts) continue;
-      const float s = a.sigmoid ? score(c[i]) : c[i] * inv_sum;
-      c[i] = key[i] == kMasked ? -INFINITY : by_score ? s + a.bias[e0 + i] : s;
-      if (by_score) key[i] = order_key(c[i]);
+      const bool masked = c[i] == (a.sigmoid ? -INFINITY : -1.0f);
+      const float s = a.sigmoid ? choice_sigmoid(c[i]) : c[i] * inv_sum;
+      c[i] = masked ? -INFINITY : s + bias[i];
+      if (by_score) key[i] = e0 + i < a.experts ? order_key(c[i]) : 0;
     }
   }
   uint32_t kept = kAll;                                           // bit g * share: group g takes part
@@ -557,7 +571,9 @@ cudaError_t launch_route_topk(const RouteArgs& args, cudaStream_t stream) {
   return by_width(a.experts, [&](auto n) {
     constexpr int kNv = decltype(n)::value;
     a.wide = whole_pieces(a.logits, a.ld_logits, a.experts, kNv, a.bf16);
-    route_topk_kernel<kNv><<<grid, kRouteWarps * 32, kRouteWarps * scratch_words(a.experts) * sizeof(uint64_t), stream>>>(a);
+    a.wide_bias = whole_pieces(a.bias, 0, a.experts, kNv, false);
+    auto kernel = a.bias != nullptr || (a.groups > 1 && a.group_top2) ? route_topk_kernel<kNv, true> : route_topk_kernel<kNv, false>;
+    kernel<<<grid, kRouteWarps * 32, kRouteWarps * scratch_words(a.experts) * sizeof(uint64_t), stream>>>(a);
   });
 }
 
