@@ -457,17 +457,23 @@ route_topk_bwd_kernel(const __grid_constant__ RouteBwdArgs a) {
   const int e0 = lane * NV;
   float s[NV];
   float top = -INFINITY;
+  // lane j holds slot j: its expert, that expert's logit and the gradient of its weight
+  const int at = lane < a.topk ? a.experts_in[token * a.topk + lane] : -1;
+  const bool valid = at >= 0 && at < a.experts;
+  float g = lane < a.topk ? a.d_weights[token * a.topk + lane] : 0.0f;
   load_logits<NV>(a.logits, token * a.ld_logits, a.experts, a.bf16, a.wide, s);
+  const float x = valid ? load_logit(a.logits, token * a.ld_logits + at, a.bf16) : 0.0f;
+  g = valid ? g * a.scale : 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) top = fmaxf(top, s[i]);
   top = warp_max(top);
   if (top == -INFINITY) top = 0.0f;
-  float sum = 0.0f;
+  float sum = 0.0f, inv_sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     if (a.sigmoid) {               // the slope s (1 - s), without the difference that cancels where s is near 1
       const float e = expf(-fabsf(s[i]));
-      s[i] = e / ((1.0f + e) * (1.0f + e));
+      s[i] = __fdividef(e, (1.0f + e) * (1.0f + e));
     } else {
       s[i] = expf(s[i] - top);
       sum += s[i];
@@ -475,18 +481,12 @@ route_topk_bwd_kernel(const __grid_constant__ RouteBwdArgs a) {
   }
   if (!a.sigmoid) {
     sum = warp_sum(sum);
+    inv_sum = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) s[i] = sum == 0.0f ? 0.0f : s[i] / sum;
+    for (int i = 0; i < NV; ++i) s[i] *= inv_sum;
   }
-  // lane j holds slot j: its expert, that expert's score and the gradient of its weight
-  const int at = lane < a.topk ? a.experts_in[token * a.topk + lane] : -1;
-  const bool valid = at >= 0 && at < a.experts;
-  float g = valid ? a.d_weights[token * a.topk + lane] * a.scale : 0.0f;
-  float mine = 0.0f;
-  if (valid) {
-    const float x = load_logit(a.logits, token * a.ld_logits + at, a.bf16);
-    mine = a.sigmoid ? 1.0f / (1.0f + expf(-x)) : sum == 0.0f ? 0.0f : expf(x - top) / sum;
-  }
+  float mine = 0.0f;                     // the score of the slot's expert
+  if (valid) mine = a.sigmoid ? 1.0f / (1.0f + expf(-x)) : expf(x - top) * inv_sum;
   if (a.renormalize) {
     const float total = warp_sum(mine), inner = warp_sum(g * mine);
     g = !valid || total == 0.0f ? 0.0f : (g - inner / total) / total;
