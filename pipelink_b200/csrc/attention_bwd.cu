@@ -156,22 +156,25 @@ struct KvWalk {
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_first() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// The waiting itself, out of the way of the roles' code. A launch finds none of its code in the instruction caches, and
+// what does not fit there is fetched again in every step: this and one copy of each product and epilogue took 2048
+// positions of 32 / 8 heads from 122 to 111 us, 2 x 4001 with a cap from 305 to 260.
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, Status* st, int code, int what) {
+  const long long t0 = clock64();
+  for (uint32_t it = 1; !mbar_try_wait(bar, parity); ++it) {
+    if ((it & 63u) != 0u) continue;
+    if (st != nullptr && ld_volatile_i32(&st->code) != 0) return false;
+    if (clock64() - t0 > kWaitBudgetCycles) {
+      if (st != nullptr) report_failure(st, code, what, parity, bar);
+      return false;
+    }
+  }
+  return true;
+}
 // A role's bounded wait; the warp's lanes agree on the outcome. Without a status record a wait that runs out goes
 // unreported, and the CTA's others run out by themselves.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, Status* st, int code, int what) {
-  bool ok = true;
-  if (!mbar_try_wait(bar, parity)) {
-    const long long t0 = clock64();
-    for (uint32_t it = 1; !mbar_try_wait(bar, parity); ++it) {
-      if ((it & 63u) != 0u) continue;
-      if (st != nullptr && ld_volatile_i32(&st->code) != 0) { ok = false; break; }
-      if (clock64() - t0 > kWaitBudgetCycles) {
-        if (st != nullptr) report_failure(st, code, what, parity, bar);
-        ok = false;
-        break;
-      }
-    }
-  }
+  const bool ok = mbar_try_wait(bar, parity) || wait_long(bar, parity, st, code, what);
   return __all_sync(kFullMask, ok) != 0;
 }
 // A compute warp's arrival: one for its 32 lanes (32 arrivals on one barrier are 32 shared-memory atomics in a row,
@@ -269,8 +272,8 @@ __device__ __forceinline__ Pair tanh_small(Pair x) {
   return mul2(x, y);
 }
 // Any x: 1 - 2 / (1 + 2^(2 x log2 e)) rather than tanh.approx, whose error the slope and the exponent would both see,
-// scaled by the cap.
-__device__ __forceinline__ float tanh_any(float x) {
+// scaled by the cap. A function of its own: 64 copies of it, hardly ever run, would lie between the code that is.
+__device__ __noinline__ float tanh_any(float x) {
   return 1.0f - __fdividef(2.0f, 1.0f + ex2_approx(fminf(x * (2.0f * kLog2e), 60.0f)));
 }
 // Probabilities of two raw scores; with a cap also its slope. minus_lse2: the rows' negated base-2 log-sum-exp; small:
@@ -475,18 +478,21 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       const int n = __shfl_sync(kFullMask, t.steps, 0), from = __shfl_sync(kFullMask, t.steps - t.blocks, 0);
       if (!warp_wait(BAR(q_full), it & 1u, p.status, ST_TIMEOUT_FULL, 412)) { ok = false; break; }
       tc_fence_after();
-      if (!issue_s(blk) || !issue_dp(blk) || (n > 1 && !issue_s(blk + 1))) { ok = false; break; }
-      if (n == 1) warp_commit(BAR(q_empty));
-      for (int j = 0; j < n && ok; ++j, ++blk) {
-        if (!warp_wait(BAR(dp_read), blk & 1u, p.status, ST_TIMEOUT_FULL, 415)) { ok = false; break; }
-        if (j + 1 < n && !issue_dp(blk + 1)) { ok = false; break; }
+      // dP(j+1), dQ(j), S(j+2), from one copy of each product's code
+      blk -= 2;
+#pragma unroll 1
+      for (int j = -2; j < n; ++j, ++blk) {
+        if (j >= 0 && !warp_wait(BAR(dp_read), blk & 1u, p.status, ST_TIMEOUT_FULL, 415)) { ok = false; break; }
+        if (j >= -1 && j + 1 < n && !issue_dp(blk + 1)) { ok = false; break; }
         if (j + 2 == n) warp_commit(BAR(q_empty));       // the last products that read Q and dO are issued: both may be replaced
-        if (!warp_wait(BAR(ds_full) + 8 * (blk & 1u), (blk >> 1) & 1u, p.status, ST_TIMEOUT_FULL, 413)) { ok = false; break; }
-        if (j == from && !warp_wait(BAR(dq_free), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_TMEM_EMPTY, 414)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t ks = blk % kDqKStages;
-        if (j < from) warp_commit(BAR(k_empty) + 8 * ks);
-        else mma_from_tmem(t_dq, t_s + (blk & 1u) * 128, sb + kDqK + ks * kTileBytes, j != from, BAR(k_empty) + 8 * ks);
+        if (j >= 0) {
+          if (!warp_wait(BAR(ds_full) + 8 * (blk & 1u), (blk >> 1) & 1u, p.status, ST_TIMEOUT_FULL, 413)) { ok = false; break; }
+          if (j == from && !warp_wait(BAR(dq_free), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_TMEM_EMPTY, 414)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t ks = blk % kDqKStages;
+          if (j < from) warp_commit(BAR(k_empty) + 8 * ks);
+          else mma_from_tmem(t_dq, t_s + (blk & 1u) * 128, sb + kDqK + ks * kTileBytes, j != from, BAR(k_empty) + 8 * ks);
+        }
         if (j + 2 < n && !issue_s(blk + 2)) { ok = false; break; }
       }
       if (!ok) break;
@@ -517,6 +523,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       if (!t.measure) {
         const size_t at = ((static_cast<size_t>(t.b) * p.seq + t.q0) * p.q_heads + t.h) * kD;
         const size_t stride = static_cast<size_t>(p.q_heads) * kD;
+#pragma unroll 1                            // code that runs once a tile is fetched as it runs: four copies took 4 us more
         for (int r0 = row0; r0 < row0 + 64; r0 += 16) {
           uint4 o[8], g[8];
 #pragma unroll
@@ -779,23 +786,28 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       const int steps = __shfl_sync(kFullMask, walk.i1 - walk.i0, 0);
       if (!warp_wait(BAR(kv_full), it & 1u, p.status, ST_TIMEOUT_FULL, 442)) { ok = false; break; }
       tc_fence_after();
-      if (!issue_s(n) || !issue_dp(n)) { ok = false; break; }
-      if (steps == 1) warp_commit(BAR(kv_empty));
-      for (int i = 0; i < steps && ok; ++i, ++n) {
+      // dV(i), S(i+1), dK(i), dP(i+1), from one copy of each product's code
+      --n;
+#pragma unroll 1
+      for (int i = -1; i < steps; ++i, ++n) {
         const bool more = i + 1 < steps;
         const uint32_t qs = n % kKvQStages, ds = n % kKvDoStages;
-        if (!warp_wait(BAR(p_full), n & 1u, p.status, ST_TIMEOUT_FULL, 443)) { ok = false; break; }
-        if (i == 0 && !warp_wait(BAR(acc_free), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_TMEM_EMPTY, 444)) { ok = false; break; }
-        tc_fence_after();
-        // dV's product starts on the half of P that is ready first
-        mma_from_tmem(t_dv, t_s, sb + kKvDo + ds * kKvStage, i != 0, 0, true, 0);
-        if (!warp_wait(BAR(p_full) + 8, n & 1u, p.status, ST_TIMEOUT_FULL, 446)) { ok = false; break; }
-        tc_fence_after();
-        mma_from_tmem(t_dv, t_s, sb + kKvDo + ds * kKvStage, true, BAR(do_empty) + 8 * ds, true, 2);
+        if (i >= 0) {
+          if (!warp_wait(BAR(p_full), n & 1u, p.status, ST_TIMEOUT_FULL, 443)) { ok = false; break; }
+          if (i == 0 && !warp_wait(BAR(acc_free), (it & 1u) ^ 1u, p.status, ST_TIMEOUT_TMEM_EMPTY, 444)) { ok = false; break; }
+          tc_fence_after();
+          // dV's product starts on the half of P that is ready first
+          mma_from_tmem(t_dv, t_s, sb + kKvDo + ds * kKvStage, i != 0, 0, true, 0);
+          if (!warp_wait(BAR(p_full) + 8, n & 1u, p.status, ST_TIMEOUT_FULL, 446)) { ok = false; break; }
+          tc_fence_after();
+          mma_from_tmem(t_dv, t_s, sb + kKvDo + ds * kKvStage, true, BAR(do_empty) + 8 * ds, true, 2);
+        }
         if (more && !issue_s(n + 1)) { ok = false; break; }
-        if (!warp_wait(BAR(ds_full), n & 1u, p.status, ST_TIMEOUT_FULL, 445)) { ok = false; break; }
-        tc_fence_after();
-        mma_from_tmem(t_dk, t_dp, sb + kKvQ + qs * kKvStage, i != 0, BAR(q_empty) + 8 * qs);
+        if (i >= 0) {
+          if (!warp_wait(BAR(ds_full), n & 1u, p.status, ST_TIMEOUT_FULL, 445)) { ok = false; break; }
+          tc_fence_after();
+          mma_from_tmem(t_dk, t_dp, sb + kKvQ + qs * kKvStage, i != 0, BAR(q_empty) + 8 * qs);
+        }
         if (more && !issue_dp(n + 1)) { ok = false; break; }
         if (i + 2 == steps) warp_commit(BAR(kv_empty));      // the last products that read K and V are issued: both may be replaced
       }
@@ -846,14 +858,6 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             if (kCap) pr[i] = mul2(pr[i], slope);
           }
         };
-        auto gradients = [&](auto m) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            Pair d = mul2(pr[i], raw(i));                                                 // and delta in dP
-            if (decltype(m)::value) d = keep_range(d, 2 * i, lo, hi);
-            pk[i] = pack_bf16(d);
-          }
-        };
         tc_ld_32x32b_x32(s_addr, v);
         tc_ld_32x32b_x32(s_addr + 32, u);
         tc_wait_ld();
@@ -876,8 +880,8 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tc_ld_32x32b_x32(dp_addr, v);
         tc_ld_32x32b_x32(dp_addr + 32, u);
         tc_wait_ld();
-        if (masked) gradients(TrueTag{});
-        else gradients(FalseTag{});
+#pragma unroll
+        for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(mul2(pr[i], raw(i)));      // delta is in dP already, masked places are 0 in pr
         tc_st_32x32b_x32(dp_addr, pk);
         tc_wait_st();
         tc_fence_before();
@@ -886,31 +890,24 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       if (!ok) break;
       if (!warp_wait(BAR(acc_full), it & 1u, p.status, ST_TIMEOUT_TMEM_FULL, 453)) { ok = false; break; }
       tc_fence_after();
-      uint32_t a[32], b[32];
-      tc_ld_32x32b_x32(t_dv + lane_addr + half * 64, a);
-      tc_ld_32x32b_x32(t_dv + lane_addr + half * 64 + 32, b);
-      tc_wait_ld();
-      if (walk.i0 == 0 && walk.i1 == t.n) {
-        const int row0 = t.k0 + quad * 32;
-        const size_t at = ((static_cast<size_t>(t.b) * p.seq + row0) * p.kv_heads + t.h) * kD + half * 64;
-        const int64_t stride = static_cast<int64_t>(p.kv_heads) * kD;
-        store_half_rows(a, b, 1.0f, p.dv + at, stride, p.seq - row0);
-        tc_ld_32x32b_x32(t_dk + lane_addr + half * 64, a);
-        tc_ld_32x32b_x32(t_dk + lane_addr + half * 64 + 32, b);
+      // dV, then dK: of a whole tile, or a part's fp32 sums for the joining kernel, 4 columns of all rows together. One
+      // copy of the code for both, as it is fetched for the first time where nothing else is left to do.
+      const bool all = walk.i0 == 0 && walk.i1 == t.n;
+      const int row0 = t.k0 + quad * 32;
+      const size_t at = ((static_cast<size_t>(t.b) * p.seq + row0) * p.kv_heads + t.h) * kD + half * 64;
+      float4* part = p.partial + (2 * static_cast<size_t>(blockIdx.x) + (walk.i0 == 0 ? 1 : 0)) * kPartVecs + half * 16 * kBlk + row;
+#pragma unroll 1
+      for (int m = 0; m < 2; ++m) {
+        uint32_t a[32], b[32];
+        tc_ld_32x32b_x32(t_dv + m * 128 + lane_addr + half * 64, a);
+        tc_ld_32x32b_x32(t_dv + m * 128 + lane_addr + half * 64 + 32, b);
         tc_wait_ld();
-        tc_fence_before();
-        warp_arrive(BAR(acc_free));
-        store_half_rows(a, b, p.scale, p.dk + at, stride, p.seq - row0);
-      } else {
-        // part of a tile: fp32 sums for the joining kernel, 4 columns of all rows together
-        float4* part = p.partial + (2 * static_cast<size_t>(blockIdx.x) + (walk.i0 == 0 ? 1 : 0)) * kPartVecs + half * 16 * kBlk + row;
-        store_part(a, b, part);
-        tc_ld_32x32b_x32(t_dk + lane_addr + half * 64, a);
-        tc_ld_32x32b_x32(t_dk + lane_addr + half * 64 + 32, b);
-        tc_wait_ld();
-        tc_fence_before();
-        warp_arrive(BAR(acc_free));
-        store_part(a, b, part + kPartVecs / 2);
+        if (m == 1) {
+          tc_fence_before();
+          warp_arrive(BAR(acc_free));
+        }
+        if (all) store_half_rows(a, b, m == 1 ? p.scale : 1.0f, (m == 1 ? p.dk : p.dv) + at, static_cast<int64_t>(p.kv_heads) * kD, p.seq - row0);
+        else store_part(a, b, part + m * (kPartVecs / 2));
       }
       ++it;
     }
