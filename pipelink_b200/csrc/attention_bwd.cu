@@ -152,7 +152,7 @@ struct KvWalk {
 };
 
 // The second kernel is launched while the first one ends: its CTAs set up on SMs that are free and wait for the first
-// one's results where they first read them (two sequences of 77: 20 us one after the other, 16 so).
+// one's results where they first read them (4 us of two sequences of 77's 20).
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_first() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -962,9 +962,9 @@ attention_bwd_join_kernel(const __grid_constant__ AttnBwdParams p, const __grid_
 // How the second kernel shares its work out. Whole tiles to CTAs leave SMs idle when there are few tiles (causal
 // tiles differ in length by their number) or the last wave is short; equal runs of steps leave none idle and cost
 // the parts' fp32 sums and the joining kernel, about ten steps' time and an eighth of what is shared out. Both kernels
-// together, whole and in runs: 2048 positions of 32 / 8 heads 155 and 126 us, 1024 of 8 / 1 heads 109 and 38 us, 4096 of
-// 32 / 8 heads 370 and 379 us.
-constexpr int kLeastSteps = 4;        // of a run: 512 positions of 8 / 2 heads take 33 us with 8, 28 with 4, 27.6 with 3
+// together, whole and in runs: 2048 positions of 32 / 8 heads 145 and 110 us, 1024 of 8 / 1 heads 106 and 36 us, 4096 of
+// 32 / 8 heads 361 and 369 us.
+constexpr int kLeastSteps = 4;        // of a run: 512 positions of 8 / 2 heads take 26.9 us with 6, 25.5 with 4, 25.1 with 3
 Runs kv_runs(int batch, int seq, int kv_heads, int group, int window) {
   const int tiles = (seq + kBlk - 1) / kBlk, bh = batch * kv_heads;
   auto length = [&](int kb) { return static_cast<int64_t>(kv_query_tiles(tiles, window, kb)) * group + kTileSteps; };
