@@ -579,7 +579,7 @@ int plb_rmsnorm_bwd(const void* d_y, int64_t ld_d_y, const void* hidden, int64_t
  * and weights_out f32 [tokens, topk], in the order of the choice. score 0: softmax over the experts, 1: sigmoid.
  * The choice goes by score + bias (f32 [experts], may be NULL), ties to the lowest index, compared as exactly as
  * fp64 allows; weights are the scores without the bias, divided by their sum over the chosen with renormalize, times
- * scale. groups > 1: experts are `groups` equal runs, a group's score is its best choice value, or the sum of its two
+ * scale (their ratios hold however small the scores are; those of exp(-700) and less are 0). groups > 1: experts are `groups` equal runs, a group's score is its best choice value, or the sum of its two
  * best with group_top2, and only the topk_groups best groups take part. A logit of -inf masks an expert: chosen
  * after every unmasked one of the kept groups, with weight 0; a token without any unmasked expert gets the lowest
  * indices and weights 0. NaN ranks below every number and spreads as the formulas say; the experts named are

@@ -106,11 +106,25 @@ __device__ __forceinline__ T warp_max(T v) {
   return v;
 }
 
-// Scaled weights of the chosen (lane j: slot j).
-__device__ __forceinline__ void store_choice(const RouteArgs& a, int64_t token, int lane, int pick, float weight) {
+// Below this sum the scores of the chosen are not divided by it: they come near the end of fp32's range, or are past it,
+// where their ratios still are of order 1. Ratios of scores are then taken from the logits, exp(x - m) with m the
+// largest chosen one (a sigmoid's 1 + exp(x) is 1 there). Above it a score that underflows is under 2^-86 of the sum.
+// Scores of exp(-700) and less, next to nothing in 64 bits too, are 0: a type's lowest number as a logit masks.
+constexpr float kFarSum = 0x1p-40f, kNoScore = -700.0f;
+// The slots' shares of their sum, from their logits and the logarithms of their scores (lane j: slot j, `in` or 0).
+__device__ __forceinline__ float far_shares(float x, float log_score, bool in) {
+  in = in && log_score > kNoScore;
+  const float m = warp_max(in ? x : -INFINITY);
+  if (m == -INFINITY) return 0.0f;
+  const float t = in ? expf(x - m) : 0.0f;
+  return t / warp_sum(t);
+}
+
+// Scaled weights of the chosen (lane j: slot j) with their logits x and scores; top: what a softmax's logits are taken from.
+__device__ __forceinline__ void store_choice(const RouteArgs& a, int64_t token, int lane, int pick, float x, float top, float weight) {
   if (a.renormalize) {
     const float total = warp_sum(lane < a.topk ? weight : 0.0f);
-    weight = total == 0.0f ? 0.0f : __fdividef(weight, total);
+    weight = total < kFarSum ? far_shares(x, a.sigmoid ? x : x - top, lane < a.topk) : __fdividef(weight, total);
   }
   if (lane < a.topk) {
     a.experts_out[token * a.topk + lane] = pick;
@@ -444,7 +458,8 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
   }
   if (count > 32) pick = exact_choice(a, token, kept, scratch);
   else if (close) pick = exact_order(a, token, pick, count);
-  store_choice(a, token, lane, pick, lane < a.topk ? score(load_logit(a.logits, token * a.ld_logits + pick, a.bf16)) : 0.0f);
+  const float x = lane < a.topk ? load_logit(a.logits, token * a.ld_logits + pick, a.bf16) : 0.0f;
+  store_choice(a, token, lane, pick, x, top, score(x));
 }
 
 template <int NV>
@@ -489,7 +504,16 @@ route_topk_bwd_kernel(const __grid_constant__ RouteBwdArgs a) {
   if (valid) mine = a.sigmoid ? 1.0f / (1.0f + expf(-x)) : expf(x - top) * inv_sum;
   if (a.renormalize) {
     const float total = warp_sum(mine), inner = warp_sum(g * mine);
-    g = !valid || total == 0.0f ? 0.0f : (g - inner / total) / total;
+    if (total < kFarSum) {
+      // dx_j = w_j (g_j - sum g w) from the shares themselves (times 1 - s for a sigmoid, which is 1), 0 for the others
+      const float w = far_shares(x, a.sigmoid ? x : x - top, valid);
+      g = w * (g - warp_sum(g * w));
+      mine = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) s[i] = s[i] * 0.0f + 1.0f;      // a NaN stays one
+    } else {
+      g = !valid ? 0.0f : (g - inner / total) / total;
+    }
   }
   const float dot = a.sigmoid ? 0.0f : warp_sum(g * mine);
   // slots to experts, in the slots' order (an expert may be named twice, which the slots' numbers find out)
