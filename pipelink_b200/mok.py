@@ -233,6 +233,7 @@ class MoKHost:
         """bf16 [E, I, H], [E, I, H], [E, H, I] for this rank's experts. ``train=True`` also
         prepares the transposed-quantised weights the data gradients contract with
         (``w_routed_*_t`` of campaigns/mok/host/resources.py:75-77)."""
+        self._forget_block()
         E, I, H = self.num_local_experts, self.shape.intermediate, self.shape.hidden
         if tuple(w_gate.shape) != (E, I, H) or tuple(w_up.shape) != (E, I, H) or tuple(w_down.shape) != (E, H, I):
             raise ValueError("weight shapes disagree with the session shape")
@@ -269,6 +270,7 @@ class MoKHost:
             self._alloc_train_buffers()
 
     def load_quantized_weights(self, gq, gsc, uq, usc, dq, dsc, keep_unpacked: bool = True):
+        self._forget_block()
         E, I, H = self.num_local_experts, self.shape.intermediate, self.shape.hidden
         w13 = torch.empty((E, 2 * I, H), dtype=torch.uint8, device=self.device)
         w13_sc = torch.empty((E * 2 * I // 128, H // 128, 32, 16), dtype=torch.uint8, device=self.device)
@@ -288,6 +290,7 @@ class MoKHost:
 
     def schedule_routes(self):
         """The schedule of the routes that already lie in ``routes_i32``."""
+        self._forget_block()
         s, sh = self.schedule, self.shape
         _lib.call("plb_moe_schedule", self.routes_i32.data_ptr(), self.world, sh.tokens, sh.topk,
                   self.rank * self.num_local_experts, self.num_local_experts, self.capacity,
@@ -562,8 +565,6 @@ class MoKHost:
         if self.weights is None:
             raise RuntimeError("load_weights() first")
         self.status.reset()
-        if self.block is not None:
-            self.block["kept"] = None       # backward_block would mix the two calls
         self.schedule_into(inputs.experts[None])
         self.x_buffer.copy_(inputs.x)
         self.router_weight_buffer.copy_(inputs.router)
@@ -599,6 +600,11 @@ class MoKHost:
                           hidden=torch.empty((sh.tokens, sh.hidden), dtype=torch.bfloat16, **on),
                           rstd=torch.empty(sh.tokens, dtype=torch.float32, **on), kept=None)
 
+    def _forget_block(self):
+        """The buffers, or the weights, are no longer those of the last forward_block(): backward_block() would mix two calls."""
+        if self.block is not None:
+            self.block["kept"] = None
+
     def forward_block(self, x: torch.Tensor, residual: torch.Tensor | None = None, *, check: bool = True, train: bool = False):
         """The expert branch of a transformer block (single rank): hidden = x + residual, its RMS norm, the router, the
         experts. x, residual bf16 [tokens, hidden]. The norm writes the tokens as the experts' dispatch takes them (bf16 and,
@@ -615,7 +621,7 @@ class MoKHost:
         if x.shape != blk["hidden"].shape or x.dtype is not torch.bfloat16 or x.device != blk["hidden"].device:
             raise ValueError("x is bf16 [tokens, hidden] on the session's device")
         self.status.reset()
-        blk["kept"] = None
+        self._forget_block()
         if residual is None:                # the session keeps the stream: x may be its own output, written again below
             x = blk["hidden"].copy_(x)
         norm.rmsnorm_fwd(x, blk["norm"], residual, eps=blk["eps"], out="both" if mx else "bf16",
