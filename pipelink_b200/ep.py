@@ -260,6 +260,9 @@ class EpMoKHost(mok.MoKHost):
             _lib.call("plb_ep_barrier", self.flags_peers.data_ptr(), self.barrier_state.data_ptr(), self.rank,
                       self.world, self.status.buf.data_ptr(), mok._stream())
 
+    def load_block(self, *args, **kwargs):
+        raise ValueError("a block's branch runs in a single-rank session (mok.MoKHost), not in a group's")
+
     def build_schedule(self):
         s, sh = self.schedule, self.shape
         if self.stream_push and self.schedule_writes_streams:

@@ -35,3 +35,16 @@ def test_no_backward_of_mixed_calls(native_lib, precision):
         host.forward_block(x, res, train=True)
         for name, value in host.backward_block(d_out).items():
             assert torch.equal(value, want[name]), name
+
+
+def test_a_groups_session_has_no_block(native_lib):
+    """Its epilogue and its dispatch read what the group's ranks pushed."""
+    from pipelink_b200 import ep, mok
+    shape = mok.Shape("group", 4, 256, 256, 2, 128)
+    group = ep.LocalGroup(shape, 1, "cuda")
+    try:
+        host = ep.EpMoKHost(shape, 0, group)
+        with pytest.raises(ValueError):
+            host.load_block(torch.ones(256), torch.zeros(4, 256))
+    finally:
+        group.close()
