@@ -13,10 +13,10 @@
 // sum has one owner: no atomics, no fp32 gradient buffer in memory and its conversion pass, the same bits in
 // every run, and gradients of shared KV heads summed in fp32 in tensor memory.
 //
-// Roundings: P and dX go to bf16 (the tensor cores' operand type, half a step 2^-9 of the value); every sum,
-// the exponent, delta and the accumulators are fp32; the gradients are rounded once when they are stored. In
-// sequences of one or two tiles, where chance would make it more, what dX loses to bf16 goes through a second product
-// (two of 77: error of dQ and dK 2.4e-3 of their norms without, 1.7e-3 with, as rounding the exact result leaves; 1.6 us).
+// Roundings: P and dX go to bf16 (the tensor cores' operand type, off by at most 2^-8 of the value); every sum,
+// the exponent, delta and the accumulators are fp32; the gradients are rounded once when they are stored. Two roundings
+// of the same size on the way, so the error of a gradient is sqrt(2) times what rounding the exact one leaves, 2.3e-3 to
+// 2.4e-3 of its norm against 1.7e-3, at any length: the errors of a sum's terms add up as the terms do.
 //
 // Tensor maps are 3-D (column, position, batch): rows past a sequence's end read as zeros and never as the
 // next sequence's, and their probabilities are forced to 0 (log-sum-exp +inf), so any length works.
@@ -77,7 +77,9 @@ __device__ __forceinline__ int snake(int wave) {
 
 // A tile of queries that see one or two key tiles (`measure`) goes over them twice, first for delta = sum P dP: where a
 // row sees few keys the rounding of the saved output is not averaged out of delta = sum dO O, and with it the error of
-// dQ and dK would be larger (sequences of 77: 2.6e-3 of the norm instead of 2.4e-3, with dX in one part).
+// dQ and dK would be larger (sequences of 20: 2.6e-3 of the norm instead of 2.3e-3, of 77: 2.5e-3 instead of 2.3e-3; a window
+// of 32 in 1024 positions: 2.44e-3 instead of 2.35e-3). It costs 0.3 us of 14 there, and where a window of at most 129 leaves
+// no other tiles, 4 to 7 % (8192 positions of 32 / 8 heads, window 64: 177 us, 165.5 without; window 128: 172 and 165).
 struct DqItem { int b, h, q0, first, blocks, steps; bool measure; };
 __device__ __forceinline__ DqItem dq_item(const AttnBwdParams& p, int w) {
   const int bh = p.batch * p.q_heads;
@@ -316,10 +318,6 @@ __device__ __forceinline__ Pair keep_range(Pair p, int i, int lo, int hi) {
   split(p, a, b);
   return make_pair(i >= lo && i < hi ? a : 0.0f, i + 1 >= lo && i + 1 < hi ? b : 0.0f);
 }
-// What pack_bf16 rounded off, as two more bf16 numbers.
-__device__ __forceinline__ uint32_t pack_rest(Pair p, uint32_t packed) {
-  return pack_bf16(fma2(make_pair(bf16_lo(packed), bf16_hi(packed)), make_pair(-1.0f, -1.0f), p));
-}
 // 64 fp32 accumulator columns of each lane's row, scaled, as bf16 to 128 bytes of the row; `rows` of the warp's rows
 // exist, `stride` elements apart from dst on. Eight lanes first exchange their 16-byte chunks so that each store
 // writes whole 128-byte pieces of four rows; a lane storing its own row would touch 32 lines with every store, some
@@ -423,7 +421,6 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(kFullMask, *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base), 0);
   const uint32_t t_dq = tmem, t_s = tmem + 128, t_dp = tmem + 384;
-  const bool few = p.tiles <= 2;          // dX in two parts
   const int items = p.tiles * p.batch * p.q_heads;
 
   if (warp == 0) {
@@ -498,12 +495,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           tc_fence_after();
           const uint32_t ks = blk % kDqKStages;
           if (j < from) warp_commit(BAR(k_empty) + 8 * ks);
-          else {
-#pragma unroll 1
-            for (int rest = 0; rest <= (few ? 1 : 0); ++rest)
-              mma_from_tmem(t_dq, t_s + (blk & 1u) * 128 + rest * 32, sb + kDqK + ks * kTileBytes, j != from || rest != 0,
-                            rest == (few ? 1 : 0) ? BAR(k_empty) + 8 * ks : 0);
-          }
+          else mma_from_tmem(t_dq, t_s + (blk & 1u) * 128, sb + kDqK + ks * kTileBytes, j != from, BAR(k_empty) + 8 * ks);
         }
         if (j + 2 < n && !issue_s(blk + 2)) { ok = false; break; }
       }
@@ -656,11 +648,6 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         if (masked) gradients(TrueTag{});
         else gradients(FalseTag{});
         tc_st_32x32b_x32(s_addr, pk);
-        if (few) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) pk[i] = pack_rest(keep_range(mul2(pr[i], add2(dp(i), minus_delta)), 2 * i, lo, hi), pk[i]);
-          tc_st_32x32b_x32(s_addr + 32, pk);
-        }
         tc_wait_st();
         tc_fence_before();
         warp_arrive(BAR(ds_full) + 8 * (blk & 1u));
@@ -737,7 +724,6 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(kFullMask, *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base), 0);
   const uint32_t t_dv = tmem, t_dk = tmem + 128, t_s = tmem + 256, t_dp = tmem + 384;
-  const bool few = p.tiles <= 2;          // dX in two parts
   const int items = p.tiles * p.batch * p.kv_heads;
 
   if (warp == 0) {
@@ -824,9 +810,7 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         if (i >= 0) {
           if (!warp_wait(BAR(ds_full), n & 1u, p.status, ST_TIMEOUT_FULL, 445)) { ok = false; break; }
           tc_fence_after();
-#pragma unroll 1
-          for (int rest = 0; rest <= (few ? 1 : 0); ++rest)
-            mma_from_tmem(t_dk, t_dp + rest * 32, sb + kKvQ + qs * kKvStage, i != 0 || rest != 0, rest == (few ? 1 : 0) ? BAR(q_empty) + 8 * qs : 0);
+          mma_from_tmem(t_dk, t_dp, sb + kKvQ + qs * kKvStage, i != 0, BAR(q_empty) + 8 * qs);
         }
         if (more && !issue_dp(n + 1)) { ok = false; break; }
         if (i + 2 == steps) warp_commit(BAR(kv_empty));      // the last products that read K and V are issued: both may be replaced
@@ -903,11 +887,6 @@ attention_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 #pragma unroll
         for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(mul2(pr[i], raw(i)));      // delta is in dP already, masked places are 0 in pr
         tc_st_32x32b_x32(dp_addr, pk);
-        if (few) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) pk[i] = pack_rest(mul2(pr[i], raw(i)), pk[i]);
-          tc_st_32x32b_x32(dp_addr + 32, pk);
-        }
         tc_wait_st();
         tc_fence_before();
         warp_arrive(BAR(ds_full));
