@@ -84,24 +84,35 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, check: b
     `pair_heads` None picks the two-heads-per-CTA kernel whenever Hq / Hkv is even. `window` > 0 adds
     the sliding-window mask (a query sees its last `window` keys), `softcap` > 0 the tanh soft cap
     on the scaled scores; both are the reference's mask / score stage variants. A sequence that is not a
-    multiple of 128 is run padded (the padding's keys lie behind every query's) and cut back."""
-    B, S, Hq, d = q.shape
-    if d != D or S < 1 or q.dtype != torch.bfloat16:
-        raise ValueError("attention_fwd wants bf16, head_dim 128 and a sequence of at least one token")
-    Hkv = k.shape[2]
-    if S % BLK:
-        q, k, v = (torch.nn.functional.pad(t, (0, 0, 0, 0, 0, BLK - S % BLK)) for t in (q, k, v))
-        out, lse = attention_fwd(q, k, v, check=check, pair_heads=pair_heads, window=window, softcap=softcap)
-        return out[:, :S].contiguous(), lse[:, :S].contiguous()
-    out = torch.empty_like(q)
-    lse = torch.empty((B * Hq, S), dtype=torch.float32, device=q.device)
-    step = heads_per_work(Hq, Hkv) if pair_heads is None else (2 if pair_heads else 1)
-    work = _device_work(B, S, Hq, step, window, q.device)   # built once per shape and device
-    status = DeviceStatus(q.device)
-    _launch(q.reshape(B * S, Hq, D), k.reshape(B * S, Hkv, D), v.reshape(B * S, Hkv, D), out.reshape(B * S, Hq, D),
-            lse, work, step, S, None, 0, status, window, softcap)
-    if check:
-        status.check("attention_fwd")
+    multiple of 128 is run padded (the padding's keys lie behind every query's) and cut back. Inputs with other
+    strides (slices of a fused projection, heads in front of positions, broadcast heads) are copied first."""
+    q_shape, kv_shape = q.shape, k.shape
+    if len(q_shape) != 4 or q_shape[3] != D or q_shape[1] < 1:
+        raise ValueError("attention_fwd wants q [B, S, Hq, 128] and a sequence of at least one token")
+    B, S, Hq, _ = q_shape
+    if len(kv_shape) != 4 or kv_shape[:2] != q_shape[:2] or kv_shape[3] != D or v.shape != kv_shape:
+        raise ValueError("attention_fwd wants k and v [B, S, Hkv, 128] beside q [B, S, Hq, 128]")
+    for t in (q, k, v):
+        if t.dtype is not torch.bfloat16 or t.device != q.device or not t.is_cuda:
+            raise ValueError("attention_fwd wants bf16 CUDA tensors on one device")
+    Hkv = kv_shape[2]
+    if Hkv == 0 or Hq == 0 or Hq % Hkv:
+        raise ValueError("the query heads must be a multiple of the KV heads")
+    with device_of(q):
+        if S % BLK:
+            q, k, v = (torch.nn.functional.pad(t, (0, 0, 0, 0, 0, BLK - S % BLK)) for t in (q, k, v))
+            out, lse = attention_fwd(q, k, v, check=check, pair_heads=pair_heads, window=window, softcap=softcap)
+            return out[:, :S].contiguous(), lse[:, :S].contiguous()
+        q, k, v = dense(q), dense(k), dense(v)
+        out = torch.empty_like(q)
+        lse = torch.empty((B * Hq, S), dtype=torch.float32, device=q.device)
+        step = heads_per_work(Hq, Hkv) if pair_heads is None else (2 if pair_heads else 1)
+        work = _device_work(B, S, Hq, step, window, q.device)   # built once per shape and device
+        status = DeviceStatus(q.device)
+        _launch(q.reshape(B * S, Hq, D), k.reshape(B * S, Hkv, D), v.reshape(B * S, Hkv, D), out.reshape(B * S, Hq, D),
+                lse, work, step, S, None, 0, status, window, softcap)
+        if check:
+            status.check("attention_fwd")
     return out, lse
 
 

@@ -22,7 +22,7 @@ import numpy as np
 import torch
 
 from . import _lib, attention
-from .mok import DeviceStatus
+from .mok import DeviceStatus, dense
 from .pipec2.launcher import Session
 
 OUT_DIR = Path(__file__).resolve().parent / "stages" / "attention" / "out"
@@ -57,6 +57,7 @@ class LinkedAttention:
         Hkv = k.shape[2]
         if d != attention.D or S % attention.BLK or q.dtype != torch.bfloat16 or attention.heads_per_work(Hq, Hkv) != 2:
             raise ValueError("the linked images are the head-pair kernel: bf16, head_dim 128, S % 128 == 0, Hq / Hkv even")
+        q, k, v = dense(q), dense(k), dense(v)
         out = torch.empty_like(q)
         lse = torch.empty((B * Hq, S), dtype=torch.float32, device=q.device)
         work = attention._device_work(B, S, Hq, 2, window, q.device)
