@@ -70,10 +70,11 @@ def zigzag_work(seq: int, world: int, rank: int, q_heads: int, step: int = 1) ->
 
 
 def _launch(q, k, v, out, lse, work, step, seq_q, ready, ready_target, status, window=0, softcap=0.0):
-    q_rows, q_heads = q.shape[0], q.shape[1]
-    kv_rows, kv_heads = k.shape[0], k.shape[1]
+    """q and out [..., q_heads, 128], k and v [..., kv_heads, 128], all dense."""
+    q_heads, kv_heads = q.shape[-2], k.shape[-2]
     _lib.call("plb_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-              work.data_ptr(), work.shape[0], step, q_heads, kv_heads, seq_q, q_rows, kv_rows, 1.0 / math.sqrt(D),
+              work.data_ptr(), work.shape[0], step, q_heads, kv_heads, seq_q, q.numel() // (q_heads * D),
+              k.numel() // (kv_heads * D), 1.0 / math.sqrt(D),
               int(window), float(softcap), 0 if ready is None else ready.data_ptr(), ready_target, status.buf.data_ptr(),
               _stream())
 
@@ -98,22 +99,28 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, check: b
     Hkv = kv_shape[2]
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError("the query heads must be a multiple of the KV heads")
+    window = _window(window)
     with device_of(q):
-        if S % BLK:
-            q, k, v = (torch.nn.functional.pad(t, (0, 0, 0, 0, 0, BLK - S % BLK)) for t in (q, k, v))
-            out, lse = attention_fwd(q, k, v, check=check, pair_heads=pair_heads, window=window, softcap=softcap)
-            return out[:, :S].contiguous(), lse[:, :S].contiguous()
+        pad = -S % BLK
+        if pad:
+            q, k, v = (torch.nn.functional.pad(t, (0, 0, 0, 0, 0, pad)) for t in (q, k, v))
         q, k, v = dense(q), dense(k), dense(v)
         out = torch.empty_like(q)
-        lse = torch.empty((B * Hq, S), dtype=torch.float32, device=q.device)
+        lse = q.new_empty((B * Hq, S + pad), dtype=torch.float32)
         step = heads_per_work(Hq, Hkv) if pair_heads is None else (2 if pair_heads else 1)
-        work = _device_work(B, S, Hq, step, window, q.device)   # built once per shape and device
+        work = _device_work(B, S + pad, Hq, step, window, q.device)   # built once per shape and device
         status = DeviceStatus(q.device)
-        _launch(q.reshape(B * S, Hq, D), k.reshape(B * S, Hkv, D), v.reshape(B * S, Hkv, D), out.reshape(B * S, Hq, D),
-                lse, work, step, S, None, 0, status, window, softcap)
+        _launch(q, k, v, out, lse, work, step, S + pad, None, 0, status, window, softcap)
         if check:
             status.check("attention_fwd")
+        if pad:
+            out, lse = out[:, :S].contiguous(), lse[:, :S].contiguous()
     return out, lse
+
+
+def _window(window: int) -> int:
+    """A window as the kernels take it, in 32 bits: a longer one hides no more than the longest."""
+    return min(window, 2 ** 31 - 1)
 
 
 def attention_bwd(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
@@ -137,6 +144,7 @@ def attention_bwd(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
             raise ValueError("attention_bwd wants bf16 CUDA tensors on one device")
     if window < 0 or not 0.0 <= softcap < math.inf:
         raise ValueError("window and softcap are 0 (off) or positive")
+    window = _window(window)
     with device_of(q):
         d_out, q, k, v, out, lse = dense(d_out), dense(q), dense(k), dense(v), dense(out), dense(lse)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)

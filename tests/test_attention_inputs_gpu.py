@@ -43,3 +43,10 @@ def test_broadcast_heads(native_lib, S):
     same(both(q, wide(k), wide(v), do), both(q, wide(k).contiguous(), wide(v).contiguous(), do))
     one = q[:, :, :1].expand(-1, -1, 4, -1)
     same(both(one, k, v, do), both(one.contiguous(), k, v, do))
+
+
+@pytest.mark.parametrize("window", [256, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5])
+def test_windows_that_hide_nothing(native_lib, window):
+    """However long: a window that does not fit in 32 bits is not cut down to what is left of it."""
+    q, k, v, do = make(1, 256, 2, 1, seed=9)
+    same(both(q, k, v, do, window=window), both(q, k, v, do))
