@@ -321,7 +321,9 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
       second = fmaxf(fmaxf(second, h), fminf(first, f));
       first = fmaxf(first, f);
     }
-    const uint32_t mine = order_key(by_sum && second > -INFINITY ? first + second : first);
+    // a sum of two as half of it, which does not overflow where a bias is near the type's end
+    if (by_sum) first = 0.5f * first + (second > -INFINITY ? 0.5f * second : 0.0f);
+    const uint32_t mine = order_key(first);
     int better = 0;
     for (int h = 0; h < a.groups; ++h) {
       const uint32_t other = __shfl_sync(kAll, mine, h << log_share);
@@ -332,8 +334,8 @@ route_topk_kernel(const __grid_constant__ RouteArgs a) {
     if (by_score || by_sum) {
       const uint32_t worst_kept = __reduce_min_sync(kAll, keep ? mine : 0xFFFFFFFFu);
       const uint32_t best_dropped = __reduce_max_sync(kAll, g < a.groups && !keep ? mine : 0u);
-      // sums of two have twice the error
-      if (near(key_value(worst_kept) * 0.5f, key_value(best_dropped) * 0.5f)) kept = exact_groups(a, token, reinterpret_cast<double*>(scratch));
+      // half a sum of two is off as much as one score
+      if (near(key_value(worst_kept), key_value(best_dropped))) kept = exact_groups(a, token, reinterpret_cast<double*>(scratch));
     }
     if (share * NV == size) {
       if (!((kept >> (g << log_share)) & 1u))
