@@ -546,9 +546,9 @@ int plb_tp_gemm_bf16(const void* a_bf16, const void* b_bf16, const int32_t* bloc
  * neither read as keys nor written). The probabilities are recomputed from lse; dk and dv are summed over the
  * query heads of their group in fp32 and rounded once, with no atomics: the same inputs give the same bits.
  * workspace: plb_attention_bwd_workspace_bytes() bytes, written and read by this call alone (its contents before and
- * after mean nothing). scale and softcap are finite, scale positive. status may be NULL: a bounded wait that runs out then goes unreported. Rows must be finite:
- * a masked pair's probability is 0, and 0 times an infinity of the pair's other operand is NaN. The reference has
- * no backward pass of its attention campaign. */
+ * after mean nothing). scale and softcap are finite, scale positive. status may be NULL: a bounded
+ * wait that runs out then goes unreported. Rows must be finite: a masked pair's probability is 0, and 0 times an
+ * infinity of the pair's other operand is NaN. The reference has no backward pass of its attention campaign. */
 size_t plb_attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv_heads, int window);
 int plb_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* d_out, const float* lse,
                       void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, int batch, int seq, int q_heads,
@@ -561,7 +561,9 @@ int plb_attention_bwd(const void* q, const void* k, const void* v, const void* o
  * [R / 128, width / 128, 32, 16] with R = rows up to a multiple of 128, rows past `rows` become zeros: the bytes of
  * plb_mxfp8_quantize on y padded with zero rows). x and residual have row strides ld_* in elements (0 repeats a
  * row), the outputs are contiguous. Any width and 2-byte alignment; 16-byte alignment throughout is faster. hidden
- * may be residual or x itself (with equal layout), no other output may overlap an input.
+ * may be residual or x itself (with equal layout), no other output may overlap an input. The squares of a row and their
+ * sum are fp32: where the sum passes 3.4e38 (numbers of 1e18 and more) rstd and y are 0, and with an eps that does not cover
+ * it, squares below 1e-38 are lost (numbers of 1e-19 and less).
  * plb_rmsnorm_bwd: d_x = rstd * (g - n * mean(g * n)) + d_hidden with g = d_y * weight, n = hidden * rstd (the
  * gradient of x and of residual alike; d_hidden, the gradient that reaches hidden past the norm, may be NULL);
  * d_weight f32 [width] = sum over rows of d_y * n, in a fixed order. hidden is what the forward pass normalised.
@@ -578,12 +580,13 @@ int plb_rmsnorm_bwd(const void* d_y, int64_t ld_d_y, const void* hidden, int64_t
  * plb_route_topk: logits [tokens, experts] (fp32, or bf16 with logits_bf16; row stride ld_logits) -> experts_out i32
  * and weights_out f32 [tokens, topk], in the order of the choice. score 0: softmax over the experts, 1: sigmoid.
  * The choice goes by score + bias (f32 [experts], may be NULL), ties to the lowest index, compared as exactly as
- * fp64 allows; weights are the scores without the bias, divided by their sum over the chosen with renormalize, times
- * scale (their ratios hold however small the scores are; those of exp(-700) and less are 0). groups > 1: experts are `groups` equal runs, a group's score is its best choice value, or the sum of its two
- * best with group_top2, and only the topk_groups best groups take part. A logit of -inf masks an expert: chosen
- * after every unmasked one of the kept groups, with weight 0; a token without any unmasked expert gets the lowest
- * indices and weights 0. NaN ranks below every number and spreads as the formulas say; the experts named are
- * always valid and distinct. experts <= 1024, topk <= 32, groups <= 32.
+ * fp64 allows; weights are the scores without the bias, divided by their sum over the chosen with renormalize (their
+ * ratios hold however small the scores are; those of exp(-700) and less are 0), times scale. groups > 1: experts are
+ * `groups` equal runs, a group's score is its best choice value, or the sum of its two best with group_top2, and only
+ * the topk_groups best groups take part. A logit of -inf masks an expert: chosen after every unmasked one of the kept
+ * groups, with weight 0; a token without any unmasked expert gets the lowest indices and weights 0. NaN ranks below
+ * every number and spreads as the formulas say; the experts named are always valid and distinct. experts <= 1024,
+ * topk <= 32, groups <= 32.
  * plb_route_topk_bwd: gradient of the weights with respect to the logits (the logits' type), for the experts that
  * were chosen; an expert that a token names twice counts twice, an index out of range not at all. The reference
  * takes routes as inputs (campaigns/mok/host/mok_port_host.py:273-282 draws them with a top-k). */

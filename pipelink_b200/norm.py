@@ -51,7 +51,8 @@ def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
                 out: str = "bf16", into: Normed | None = None) -> Normed:
     """x, residual bf16 [..., width], weight bf16 [width]. `out`: "bf16", "mxfp8" (width a multiple of 128) or "both".
     hidden = bf16(x + residual), y = bf16(hidden * rstd * weight). `into` gives the tensors to write (contiguous; those of
-    an earlier call of the same shape, or a session's buffers) instead of new ones; its hidden may be the residual itself."""
+    an earlier call of the same shape, or a session's buffers) instead of new ones; its hidden may be the residual itself.
+    A row's squares and their sum are fp32: where the sum passes 3.4e38 (numbers of 1e18 and more) y is 0."""
     if out not in ("bf16", "mxfp8", "both"):
         raise ValueError("out is 'bf16', 'mxfp8' or 'both'")
     width, dev = _check(weight, x, residual)
