@@ -546,7 +546,7 @@ int plb_tp_gemm_bf16(const void* a_bf16, const void* b_bf16, const int32_t* bloc
  * neither read as keys nor written). The probabilities are recomputed from lse; dk and dv are summed over the
  * query heads of their group in fp32 and rounded once, with no atomics: the same inputs give the same bits.
  * workspace: plb_attention_bwd_workspace_bytes() bytes, written and read by this call alone (its contents before and
- * after mean nothing). scale and softcap are finite, scale positive. status may be NULL: a bounded
+ * after mean nothing). scale is from 2^-96 to 2^96, softcap at most 2^96. status may be NULL: a bounded
  * wait that runs out then goes unreported. Rows must be finite: a masked pair's probability is 0, and 0 times an
  * infinity of the pair's other operand is NaN. The reference has no backward pass of its attention campaign. */
 size_t plb_attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv_heads, int window);

@@ -1035,8 +1035,9 @@ size_t plb_attention_bwd_workspace_bytes(int batch, int seq, int q_heads, int kv
 int plb_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* d_out, const float* lse,
                       void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, int batch, int seq, int q_heads,
                       int kv_heads, float scale, int window, float softcap, plb_status* status, void* stream) {
-  if (!attention_bwd_shape_ok(batch, seq, q_heads, kv_heads, window) || !(scale >= FLT_MIN && scale <= FLT_MAX)) return PLB_E_ARGUMENT;
-  if (!(softcap >= 0.0f && softcap <= FLT_MAX) || (softcap > 0.0f && scale / softcap > FLT_MAX)) return PLB_E_ARGUMENT;
+  // the log-sum-exp is divided by the scale, and the cap multiplied by log2 e, in fp32: both have to stay numbers
+  if (!attention_bwd_shape_ok(batch, seq, q_heads, kv_heads, window) || !(scale >= 0x1p-96f && scale <= 0x1p96f)) return PLB_E_ARGUMENT;
+  if (!(softcap >= 0.0f && softcap <= 0x1p96f) || (softcap > 0.0f && scale / softcap > FLT_MAX)) return PLB_E_ARGUMENT;
   if (batch == 0 || seq == 0) return PLB_OK;
   if (!q || !k || !v || !out || !d_out || !lse || !dq || !dk || !dv || !workspace) return PLB_E_ARGUMENT;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(d_out) || !aligned16(dq) ||
