@@ -620,28 +620,29 @@ class MoKHost:
         blk, mx = self.block, self.precision == "mxfp8"
         if x.shape != blk["hidden"].shape or x.dtype is not torch.bfloat16 or x.device != blk["hidden"].device:
             raise ValueError("x is bf16 [tokens, hidden] on the session's device")
-        self.status.reset()
-        self._forget_block()
-        if residual is None:                # the session keeps the stream: x may be its own output, written again below
-            x = blk["hidden"].copy_(x)
-        norm.rmsnorm_fwd(x, blk["norm"], residual, eps=blk["eps"], out="both" if mx else "bf16",
-                         into=norm.Normed(blk["hidden"], blk["rstd"], self.x_buffer, self.xq if mx else None, self.xsc if mx else None))
-        if mx:
-            self.token_scale_rows()
-        blk["logits"] = torch.mm(self.x_buffer, blk["gate"].T, out_dtype=torch.float32)
-        router.route_topk(blk["logits"], self.shape.topk, bias=blk["bias"], into=(self.routes_i32, self.router_weight_buffer),
-                          **blk["routing"])
-        self.schedule_routes()
-        self.pull()
-        if train:
-            self.gemm_gate_up_train()
-        else:
-            self.gemm_gate_up()
-        self.gemm_down()
-        out = self.fwd_epilogue()
-        blk["kept"] = "train" if train else "recompute"
-        if check:
-            self.status.check("after a block's forward pass")
+        with device_of(x):
+            self.status.reset()
+            self._forget_block()
+            if residual is None:                # the session keeps the stream: x may be its own output, written again below
+                x = blk["hidden"].copy_(x)
+            norm.rmsnorm_fwd(x, blk["norm"], residual, eps=blk["eps"], out="both" if mx else "bf16",
+                             into=norm.Normed(blk["hidden"], blk["rstd"], self.x_buffer, self.xq if mx else None, self.xsc if mx else None))
+            if mx:
+                self.token_scale_rows()
+            blk["logits"] = torch.mm(self.x_buffer, blk["gate"].T, out_dtype=torch.float32)
+            router.route_topk(blk["logits"], self.shape.topk, bias=blk["bias"], into=(self.routes_i32, self.router_weight_buffer),
+                              **blk["routing"])
+            self.schedule_routes()
+            self.pull()
+            if train:
+                self.gemm_gate_up_train()
+            else:
+                self.gemm_gate_up()
+            self.gemm_down()
+            out = self.fwd_epilogue()
+            blk["kept"] = "train" if train else "recompute"
+            if check:
+                self.status.check("after a block's forward pass")
         return {"output": out, "hidden": blk["hidden"], "experts": self.routes_i32[0], "router": self.router_weight_buffer,
                 "logits": blk["logits"], **self.context_tensors()}
 
@@ -657,14 +658,15 @@ class MoKHost:
             raise RuntimeError("forward_block(train=True) first, or recompute=True")
         if d_out.shape != blk["hidden"].shape or d_out.dtype is not torch.bfloat16 or d_out.device != blk["hidden"].device:
             raise ValueError("d_out is bf16 [tokens, hidden] on the session's device")
-        g = self.backward(dense(d_out), check=False, recompute=recompute)
-        routing = {k: v for k, v in blk["routing"].items() if k in ("score", "renormalize", "scale")}
-        d_logits = router.route_topk_bwd(g["d_router_weights"], blk["logits"], self.routes_i32[0], **routing)
-        d_y = torch.addmm(g["d_x"].float(), d_logits, blk["gate"].float()).to(torch.bfloat16)
-        d_x, d_norm = norm.rmsnorm_bwd(d_y, blk["hidden"], blk["rstd"], blk["norm"], d_hidden)
-        if check:
-            self.status.check("after a block's backward pass")
-        return {**g, "d_x": d_x, "d_norm_weight": d_norm, "d_gate_weight": d_logits.T @ self.x_buffer.float()}
+        with device_of(d_out):
+            g = self.backward(dense(d_out), check=False, recompute=recompute)
+            routing = {k: v for k, v in blk["routing"].items() if k in ("score", "renormalize", "scale")}
+            d_logits = router.route_topk_bwd(g["d_router_weights"], blk["logits"], self.routes_i32[0], **routing)
+            d_y = torch.addmm(g["d_x"].float(), d_logits, blk["gate"].float()).to(torch.bfloat16)
+            d_x, d_norm = norm.rmsnorm_bwd(d_y, blk["hidden"], blk["rstd"], blk["norm"], d_hidden)
+            if check:
+                self.status.check("after a block's backward pass")
+            return {**g, "d_x": d_x, "d_norm_weight": d_norm, "d_gate_weight": d_logits.T @ self.x_buffer.float()}
 
     def host_pipeline(self):
         """A forward loop over HOST buffers (see HostPipeline)."""
