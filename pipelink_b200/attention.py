@@ -34,7 +34,7 @@ def heads_per_work(q_heads: int, kv_heads: int) -> int:
     return 2 if (q_heads // kv_heads) % 2 == 0 else 1
 
 
-@functools.lru_cache(maxsize=64)
+@functools.lru_cache(maxsize=None)      # a captured graph reads the list of its shape for as long as it lives
 def _device_work(batch, seq, q_heads, step, window, device):
     return torch.from_numpy(causal_work(batch, seq, q_heads, step, window)).to(device)
 
