@@ -102,9 +102,9 @@ struct RowTeam {
   }
 };
 
-// NV chunks of VEC elements a thread. Threads per SM by what a thread holds, the registers it needs without spilling:
-// 2048 for 8 elements (16384 x 2048: 44 us with one register more, 41 so), 1280 for 16 (16384 x 4096 with both outputs:
-// 100 us with 1024, 91 so), 1024 for 32.
+// NV chunks of VEC elements a thread. Threads per SM by what a thread holds, with the registers that suffice but for a
+// few words (8 bytes a thread of 32 elements in a warp's row, 6 to 10 of single ones): 2048 for 8 elements (16384 x 2048: 44
+// us with one register more, 41 so), 1280 for 16 (16384 x 4096 with both outputs: 100 us with 1024, 91 so), 1024 for 32.
 template <int VEC, int SIZE, int NV>
 __global__ void __launch_bounds__(RowTeam<SIZE>::kThreads, (NV * VEC <= 8 ? 2048 : NV * VEC <= 16 ? 1280 : 1024) / RowTeam<SIZE>::kThreads)
 rmsnorm_fwd_rows(const __grid_constant__ NormFwdArgs a) {
@@ -204,7 +204,8 @@ rmsnorm_fwd_rows(const __grid_constant__ NormFwdArgs a) {
 // the CTA walks, so dy and h are read once for both.
 //
 // CTAs per SM: 1024 threads where a thread holds 8 elements, 512 (128 registers) where it holds more or loads ahead; 768
-// threads of 16 elements spill (16384 x 4096: 114 us, with 512 threads 104).
+// threads of 16 elements spill (16384 x 4096: 114 us, with 512 threads 104). Rows of 8200 to 16384 (32 elements and their sums a
+// thread) spill 280 bytes a thread, rows of 520 to 1024 in a warp 108 (4096 x 16384: 125 us, 0.66 of the copy rate).
 template <int VEC, int SIZE, int NV>
 constexpr int kBwdResident = SIZE == 1024 ? 1 : (SIZE == 32 || NV * VEC > 8 ? 512 : 1024) / RowTeam<SIZE>::kThreads;
 template <int VEC, int SIZE, int NV>

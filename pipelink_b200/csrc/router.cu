@@ -7,7 +7,7 @@
 //
 // One warp per token, NV consecutive experts to a lane. The topk-th largest of the 32 lanes' maxima bounds the topk-th
 // value from below: what is not under it, some 10 to 20 candidates, is put one to a lane and ranked by comparing each
-// with each (16384 tokens, 256 experts, 8 chosen: 11.4 us; rounds of maxima took 7 us more). Where that leaves
+// with each (16384 tokens, 256 experts, 8 chosen: 11.6 us; rounds of maxima took 7 us more). Where that leaves
 // more than 32 (many ties, a large topk), topk rounds of a warp-wide maximum choose. Without a bias the scores are
 // ordered as the logits are, and those are compared as they stand. With one (or with sums of two scores over groups) the
 // order is that of numbers fp32 may not tell apart. Every comparison that matters is checked against the bound of the
@@ -229,7 +229,7 @@ __device__ __noinline__ int exact_choice(const RouteArgs& a, int64_t token, uint
 }
 
 // kScored: the choice needs the scores, for a bias or the sums of two; without them no comparison is ever close, and the
-// kernel has neither the tests nor the fp64 paths (65536 x 128: 33 us with them, 28 without).
+// kernel has neither the tests nor the fp64 paths (65536 x 128: 37.7 us with them, 31.6 without).
 //
 // CTAs per SM: what hides the latencies of a token's steps is other tokens, at the price of registers where a lane
 // holds few experts (256 experts in groups with a bias: 18.1 us with 40 warps an SM, 18.5 with 48; by logits alone 48 are
