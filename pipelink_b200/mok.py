@@ -605,6 +605,7 @@ class MoKHost:
         if self.block is not None:
             self.block["kept"] = None
 
+    @torch.no_grad()
     def forward_block(self, x: torch.Tensor, residual: torch.Tensor | None = None, *, check: bool = True, train: bool = False):
         """The expert branch of a transformer block (single rank): hidden = x + residual, its RMS norm, the router, the
         experts. x, residual bf16 [tokens, hidden]. The norm writes the tokens as the experts' dispatch takes them (bf16 and,
@@ -646,6 +647,7 @@ class MoKHost:
         return {"output": out, "hidden": blk["hidden"], "experts": self.routes_i32[0], "router": self.router_weight_buffer,
                 "logits": blk["logits"], **self.context_tensors()}
 
+    @torch.no_grad()
     def backward_block(self, d_out: torch.Tensor, d_hidden: torch.Tensor | None = None, *, check: bool = True, recompute: bool = False):
         """Backward of the last ``forward_block(train=True)`` (or of a plain one with ``recompute``): `d_out` is the gradient of
         "output", `d_hidden` what reaches "hidden" from behind. Returns d_x (of x and of the residual alike), d_norm_weight,

@@ -48,3 +48,16 @@ def test_a_groups_session_has_no_block(native_lib):
             host.load_block(torch.ones(256), torch.zeros(4, 256))
     finally:
         group.close()
+
+
+def test_nothing_is_recorded_for_autograd(native_lib):
+    """Inputs that want gradients leave none of autograd's records in the session's buffers: the gradients are
+    backward_block's, and a record would grow with every call."""
+    host, w, x, res, d_out = session(("leaf", 4, 256, 256, 2, 160), "bf16", train=True)
+    want = host.forward_block(x, train=True)["output"].clone()
+    leaf = x.clone().requires_grad_(True)
+    for residual in (None, res.clone().requires_grad_(True)):
+        got = host.forward_block(leaf, residual, train=True)
+        assert not any(t.requires_grad for t in got.values()) and not host.block["hidden"].requires_grad
+        assert residual is not None or torch.equal(got["output"], want)
+        assert not any(t.requires_grad for t in host.backward_block(d_out.clone().requires_grad_(True)).values())
